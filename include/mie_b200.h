@@ -46,6 +46,7 @@ extern "C" {
 #define MIE_STATUS_NO_TOKEN 128      /* greedy sampling saw no candidate for a row; token 0 was written */
 #define MIE_STATUS_BAD_TOKEN 256     /* token id outside the vocabulary (row 0 was used) */
 #define MIE_STATUS_BAD_SLOT 512      /* state slot outside the state buffer (the row was skipped) */
+#define MIE_STATUS_BAD_EXPERT 1024   /* expert id outside the pool and not -1 (the choice was skipped) */
 
 /* Element types of K/V pages, queries and activations. */
 #define MIE_DTYPE_BF16 0
@@ -481,6 +482,53 @@ int mie_lm_head_argmax(const void* x, int64_t ldx, const void* w, int64_t ldw, i
 #define MIE_LINEAR_NO_WEIGHT_PREFETCH 4
 int mie_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, void* y, int64_t ldy,
                int32_t m, int32_t n, int32_t k, int32_t kernel, int32_t* status, void* stream);
+
+/* Activations of fused projections and feed-forwards: z, z / (1 + exp(-z)), the tanh form of gelu, max(z, 0). */
+#define MIE_ACT_NONE 0
+#define MIE_ACT_SILU 1
+#define MIE_ACT_GELU 2
+#define MIE_ACT_RELU 3
+
+/*
+ * Projection of bf16 rows with its epilogue: y[m, n] = act(x[m, k] w[n, k]^T + bias[n]) + residual[m, n]; gated: w and
+ * bias have 2 n rows, gates first, and y = act(x w_g^T + bias_g) * (x w_u^T + bias_u) + residual.  fp32 sums and epilogue,
+ * one rounding to bf16.  bias and residual may be NULL; y may be the residual itself, not x.  Strides in elements, any
+ * sizes and alignments.
+ */
+int mie_fused_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
+                     int64_t ldr, void* y, int64_t ldy, int32_t m, int32_t n, int32_t k, int32_t activation,
+                     int32_t gated, int32_t* status, void* stream);
+
+/*
+ * Experts of every token, from its router logits z[experts] (bf16, fp16 or fp32 by `dtype`, row stride `ld`):
+ * s = softmax(z) or sigmoid(z), c = s + bias[experts] (fp32, may be NULL), -inf where z is -inf.  With groups > 1, the
+ * experts are that many equal runs; the top_groups groups whose group_best (1 or 2) largest c add up to most stay.
+ * ids[tokens, top_k]: the experts with the largest c, descending, equal ones by their index, as 64 bits decide;
+ * weights: s of those, over their sum if `renormalize` (0 if that is 0), times scale.  A token with a NaN among its
+ * logits gets NaN weights.
+ */
+#define MIE_SCORES_SOFTMAX 0
+#define MIE_SCORES_SIGMOID 1
+#define MIE_MAX_EXPERTS 1024
+#define MIE_MAX_TOP_K 32
+int mie_route_experts(const void* logits, int64_t ld, int32_t dtype, const float* bias, int32_t scores, int32_t tokens,
+                      int32_t experts, int32_t top_k, int32_t groups, int32_t top_groups, int32_t group_best,
+                      int32_t renormalize, float scale, int32_t* ids, float* weights, void* stream);
+
+/*
+ * Gated feed-forward of routed experts: y[t] = residual[t] + sum_j weights[t, j] D_e (act(G_e x[t]) * (U_e x[t])) with
+ * e = ids[t, j]; gate_up[e] = [G_e; U_e] is [2 ff, width], down[e] = D_e is [width, ff], bf16, strides in elements.
+ * weights: contiguous fp32 [tokens, top_k].  An id of -1 is no expert; others outside [0, experts) are skipped and
+ * reported (MIE_STATUS_BAD_EXPERT).  fp32 sums; the gated rows are rounded once to bf16 (with their weight) before the
+ * down product, y once.  y may be the residual itself, not x.  scratch: mie_expert_scratch_bytes of device memory,
+ * 256-byte aligned, in use until the call's work is done.
+ */
+int64_t mie_expert_scratch_bytes(int32_t tokens, int32_t top_k, int32_t experts, int32_t width, int32_t ff);
+int mie_expert_mlp(const void* x, int64_t ldx, mie_index_t ids, const float* weights, const void* gate_up,
+                   int64_t gate_up_row, int64_t gate_up_expert, const void* down, int64_t down_row, int64_t down_expert,
+                   const void* residual, int64_t ldr, void* y, int64_t ldy, int32_t tokens, int32_t top_k,
+                   int32_t experts, int32_t width, int32_t ff, int32_t activation, void* scratch, int64_t scratch_bytes,
+                   int32_t* status, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Tensor-parallel exchange (no counterpart in the reference, which runs on one

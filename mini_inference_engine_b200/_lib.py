@@ -6,6 +6,7 @@ loaded, every operator of this package raises ``MieLibraryError``.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int32, c_int64, c_void_p
@@ -25,6 +26,7 @@ STATUS_CAPACITY = 64
 STATUS_NO_TOKEN = 128
 STATUS_BAD_TOKEN = 256
 STATUS_BAD_SLOT = 512
+STATUS_BAD_EXPERT = 1024
 
 GEMM_NO_WEIGHT_PREFETCH = 1
 GEMM_STATIC_WEIGHTS = 2
@@ -40,6 +42,7 @@ STATUS_MESSAGES = {
     STATUS_NO_TOKEN: "greedy sampling found no candidate for a row (token 0 was substituted)",
     STATUS_BAD_TOKEN: "a token id lies outside the vocabulary",
     STATUS_BAD_SLOT: "a state slot lies outside the state buffer",
+    STATUS_BAD_EXPERT: "an expert id lies outside the expert pool",
 }
 
 DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -140,6 +143,14 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                           c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "mie_linear": (ctypes.c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int32, c_int32,
                                   c_int32, c_int32, c_void_p, c_void_p]),
+    "mie_fused_linear": (ctypes.c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p,
+                                        c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p]),
+    "mie_route_experts": (ctypes.c_int, [c_void_p, c_int64, c_int32, c_void_p, c_int32, c_int32, c_int32, c_int32,
+                                         c_int32, c_int32, c_int32, c_int32, c_float, c_void_p, c_void_p, c_void_p]),
+    "mie_expert_scratch_bytes": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32]),
+    "mie_expert_mlp": (ctypes.c_int, [c_void_p, c_int64, IndexT, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+                                      c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32,
+                                      c_int32, c_int32, c_void_p, c_int64, c_void_p, c_void_p]),
     "mie_ipc_export": (ctypes.c_int, [c_void_p, c_void_p, ctypes.POINTER(c_int64)]),
     "mie_ipc_open": (ctypes.c_int, [c_void_p, c_int64, ctypes.POINTER(c_void_p)]),
     "mie_ipc_close": (ctypes.c_int, [c_void_p, c_int64]),
@@ -284,6 +295,15 @@ def view4_arg(tensor: torch.Tensor | None) -> View4T:
 
 def stream_arg(device: torch.device | None = None) -> c_void_p:
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context in which launches go to ``device``, which need not be the current one."""
+
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def ptr(tensor: torch.Tensor | None) -> c_void_p:

@@ -1,0 +1,242 @@
+// The gated feed-forward of routed experts:
+//
+//   y[t] = res[t] + sum_j w[t, j] D_e (act(G_e x[t]) * (U_e x[t])),   e = ids[t, j]
+//
+//   expert_plan_kernel     sorts the (token, choice) pairs by expert and cuts every expert's rows into tiles
+//   gate and up product    rows of x gathered by pair, activation, gate and the pair's weight in the epilogue
+//   down product           one row of sums per pair, in the pairs' own order
+//   expert_combine_kernel  adds a token's rows and the residual
+//
+// A pair's order among its expert's rows is whatever the counters gave; every row of a product is computed by itself, so
+// the results do not depend on it.  Ids outside [0, experts) take no part: -1 says "no expert", others also set a status bit.
+#include "products.cuh"
+
+namespace mie {
+namespace {
+
+struct PlanParams {
+  IndexView ids;  // [tokens, top_k]
+  int pairs, top_k, experts, tile_rows;
+  int* order;     // [pairs] sorted row -> pair
+  RowTile* tiles;
+  int* tile_count;
+  int* status;
+};
+
+constexpr int kPlanThreads = 1024;
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void plan_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int ld_cluster_int(const int* local, uint32_t rank) {
+  uint32_t remote;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(local)), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
+  return v;
+}
+
+// Sum of `v` over the threads before this one; one value per thread, at most 1024 threads.
+__device__ __forceinline__ int block_scan_before(int v, int* warp_sums) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int sum = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int other = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += other;
+  }
+  if (lane == 31) warp_sums[warp] = sum;
+  __syncthreads();
+  if (warp == 0) {
+    int s = lane < (int)(blockDim.x >> 5) ? warp_sums[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += other;
+    }
+    warp_sums[lane] = s;
+  }
+  __syncthreads();
+  const int before = (warp > 0 ? warp_sums[warp - 1] : 0) + sum - v;
+  __syncthreads();  // warp_sums may be used again
+  return before;
+}
+
+// One cluster.  Every CTA counts its part of the pairs by expert in shared memory; a thread per expert adds the parts up, and
+// with the offsets from a scan over the experts the pairs get their places.
+__global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const PlanParams p) {
+  __shared__ int count[MIE_MAX_EXPERTS], place[MIE_MAX_EXPERTS], warp_sums[32];
+  const uint32_t rank = cluster_rank(), ranks = gridDim.x;
+  const int begin = (int)((long long)p.pairs * rank / ranks), end = (int)((long long)p.pairs * (rank + 1) / ranks);
+  chain_release();
+  for (int e = threadIdx.x; e < p.experts; e += kPlanThreads) count[e] = 0;
+  __syncthreads();
+  chain_wait();
+  for (int i = begin + threadIdx.x; i < end; i += kPlanThreads) {
+    const long long e = p.ids.at(i / p.top_k, i % p.top_k);
+    if (e >= 0 && e < p.experts)
+      atomicAdd(&count[e], 1);
+    else if (e != -1)
+      raise_status(p.status, MIE_STATUS_BAD_EXPERT);
+  }
+  plan_cluster_sync();
+  const int e = threadIdx.x;
+  int total = 0, before = 0;
+  if (e < p.experts) {
+    for (uint32_t r = 0; r < ranks; ++r) {
+      const int c = ld_cluster_int(&count[e], r);
+      if (r < rank) before += c;
+      total += c;
+    }
+  }
+  const int first = block_scan_before(total, warp_sums);
+  if (e < p.experts) place[e] = first + before;
+  if (rank == 0) {
+    const int tiles = (total + p.tile_rows - 1) / p.tile_rows;
+    const int tile = block_scan_before(tiles, warp_sums);
+    for (int i = 0; i < tiles; ++i) {
+      const int left = total - i * p.tile_rows;
+      p.tiles[tile + i] = RowTile{e, first + i * p.tile_rows, left < p.tile_rows ? left : p.tile_rows, 0};
+    }
+    if (e == kPlanThreads - 1) *p.tile_count = tile + tiles;
+  }
+  __syncthreads();
+  for (int i = begin + threadIdx.x; i < end; i += kPlanThreads) {
+    const long long expert = p.ids.at(i / p.top_k, i % p.top_k);
+    if (expert >= 0 && expert < p.experts) p.order[atomicAdd(&place[expert], 1)] = i;
+  }
+  plan_cluster_sync();  // no CTA leaves while another may still read its counts
+}
+
+struct CombineParams {
+  const float* rows;  // [tokens * top_k, width]
+  IndexView ids;
+  const __nv_bfloat16* residual;
+  long long ldr;
+  __nv_bfloat16* y;
+  long long ldy;
+  int tokens, top_k, width, experts;
+};
+
+// Adds in the order of the choices.
+__global__ void __launch_bounds__(256) expert_combine_kernel(const CombineParams p) {
+  chain_release();
+  chain_wait();
+  const long long total = (long long)p.tokens * p.width;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+    const long long t = i / p.width;
+    const int c = (int)(i - t * p.width);
+    float sum = p.residual != nullptr ? __bfloat162float(p.residual[t * p.ldr + c]) : 0.f;
+    for (int j = 0; j < p.top_k; ++j) {
+      const long long e = p.ids.at(t, j);
+      if (e >= 0 && e < p.experts) sum += p.rows[(t * p.top_k + j) * p.width + c];
+    }
+    p.y[t * p.ldy + c] = __float2bfloat16_rn(sum);
+  }
+}
+
+// Where the parts of the scratch begin.
+struct Scratch {
+  long long order, tiles, tile_count, hidden, rows, total;
+  long long max_tiles;
+  Scratch(long long pairs, int experts, int width, int ff, int tile_rows) {
+    auto take = [this](long long bytes) {
+      const long long at = total;
+      total += (bytes + 255) / 256 * 256;
+      return at;
+    };
+    total = 0;
+    max_tiles = pairs / tile_rows + (pairs < experts ? pairs : experts);
+    order = take(pairs * 4);
+    tiles = take(max_tiles * (long long)sizeof(RowTile));
+    tile_count = take(4);
+    hidden = take(pairs * ff * 2);
+    rows = take(pairs * width * 4);
+  }
+};
+
+}  // namespace
+}  // namespace mie
+
+using namespace mie;
+
+extern "C" int64_t mie_expert_scratch_bytes(int32_t tokens, int32_t top_k, int32_t experts, int32_t width, int32_t ff) {
+  if (tokens < 0 || top_k < 1 || experts < 1 || width < 1 || ff < 1) return 0;
+  return Scratch((long long)tokens * top_k, experts, width, ff, kAnyTile).total;
+}
+
+extern "C" int mie_expert_mlp(const void* x, int64_t ldx, mie_index_t ids, const float* weights, const void* gate_up,
+                              int64_t gate_up_row, int64_t gate_up_expert, const void* down, int64_t down_row,
+                              int64_t down_expert, const void* residual, int64_t ldr, void* y, int64_t ldy,
+                              int32_t tokens, int32_t top_k, int32_t experts, int32_t width, int32_t ff,
+                              int32_t activation, void* scratch, int64_t scratch_bytes, int32_t* status, void* stream_) {
+  cudaStream_t stream = (cudaStream_t)stream_;
+  MIE_CHECK_ARG(x && ids.ptr && weights && gate_up && down && y && scratch, "null pointer");
+  MIE_CHECK_ARG(tokens >= 0 && width >= 1 && ff >= 1 && experts >= 1 && experts <= MIE_MAX_EXPERTS && top_k >= 1 &&
+                    top_k <= MIE_MAX_TOP_K,
+                "invalid sizes: %d tokens of %d, %d of %d experts of %d", tokens, width, top_k, experts, ff);
+  MIE_CHECK_ARG((long long)tokens * top_k < (1ll << 30), "too many (token, expert) pairs");
+  MIE_CHECK_ARG(ldx >= width && gate_up_row >= width && down_row >= ff && ldy >= width && (!residual || ldr >= width),
+                "a row is longer than its stride");
+  MIE_CHECK_ARG(activation >= MIE_ACT_NONE && activation <= MIE_ACT_RELU, "unknown activation %d", activation);
+  const int pairs = tokens * top_k;
+  const Scratch s(pairs, experts, width, ff, kAnyTile);
+  MIE_CHECK_ARG(scratch_bytes >= s.total, "scratch of %lld bytes, %lld needed", (long long)scratch_bytes, s.total);
+  if (tokens == 0) return MIE_OK;
+  uint8_t* base = (uint8_t*)scratch;
+  int* order = (int*)(base + s.order);
+
+  PlanParams plan{IndexView(ids), pairs, top_k, experts, kAnyTile, order, (RowTile*)(base + s.tiles),
+                  (int*)(base + s.tile_count), status};
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(pairs > 4096 ? 8 : 1);
+  config.blockDim = dim3(kPlanThreads);
+  config.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = config.gridDim.x;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = chained_launch_enabled() ? 2 : 1;
+  MIE_CUDA(cudaLaunchKernelEx(&config, expert_plan_kernel, plan));
+  MIE_LAUNCH_CHECK("expert_plan_kernel");
+
+  Product up = {};
+  up.x = (const __nv_bfloat16*)x, up.ldx = ldx;
+  up.w = (const __nv_bfloat16*)gate_up, up.ldw = gate_up_row, up.w_expert = gate_up_expert;
+  up.y = base + s.hidden, up.ldy = ff;
+  up.m = pairs, up.n = ff, up.k = width;
+  up.activation = activation, up.gated = 1, up.status = status;
+  up.tiles = plan.tiles, up.tile_count = plan.tile_count;
+  up.source = order, up.source_divisor = top_k, up.factor = weights;
+  const unsigned tiles = (unsigned)(s.max_tiles < 65535 ? s.max_tiles : 65535);
+  MIE_CUDA(launch_chained(product_any_kernel<true>, dim3((unsigned)((ff + kAnyTile - 1) / kAnyTile), tiles), dim3(128), 0,
+                          stream, up));
+  MIE_LAUNCH_CHECK("product_any_kernel");
+
+  Product out = {};
+  out.x = (const __nv_bfloat16*)(base + s.hidden), out.ldx = ff;
+  out.w = (const __nv_bfloat16*)down, out.ldw = down_row, out.w_expert = down_expert;
+  out.y = base + s.rows, out.ldy = width, out.wide = 1;
+  out.m = pairs, out.n = width, out.k = ff;
+  out.status = status;
+  out.tiles = plan.tiles, out.tile_count = plan.tile_count, out.target = order;
+  MIE_CUDA(launch_chained(product_any_kernel<true>, dim3((unsigned)((width + kAnyTile - 1) / kAnyTile), tiles), dim3(128), 0,
+                          stream, out));
+  MIE_LAUNCH_CHECK("product_any_kernel");
+
+  const CombineParams combine{(const float*)(base + s.rows), IndexView(ids), (const __nv_bfloat16*)residual, ldr,
+                              (__nv_bfloat16*)y, ldy, tokens, top_k, width, experts};
+  const long long blocks = ((long long)tokens * width + 255) / 256, most = 16ll * sm_count();
+  MIE_CUDA(launch_chained(expert_combine_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream,
+                          combine));
+  MIE_LAUNCH_CHECK("expert_combine_kernel");
+  return MIE_OK;
+}

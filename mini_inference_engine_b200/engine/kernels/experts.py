@@ -1,0 +1,98 @@
+"""Routed feed-forwards: the choice of every token's experts (``csrc/expert_routing.cu``) and the experts' products
+(``csrc/expert_mlp.cu``)."""
+
+from __future__ import annotations
+
+import torch
+
+from ... import _lib
+from .linear import activation_code, check_rows, row_stride
+
+MAX_EXPERTS = 1024  # MIE_MAX_EXPERTS
+MAX_TOP_K = 32      # MIE_MAX_TOP_K
+SCORES = {"softmax": 0, "sigmoid": 1}  # MIE_SCORES_*
+
+
+def route_experts(logits: torch.Tensor, top_k: int, *, scores: str = "softmax", bias: torch.Tensor | None = None,
+                  groups: int = 1, top_groups: int = 1, group_best: int = 1, renormalize: bool = True,
+                  scale: float = 1.0, status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(ids int32 [tokens, top_k], weights fp32 [tokens, top_k])`` of router logits ``[tokens, experts]`` (bf16, fp16 or
+    fp32).
+
+    ``s = softmax(logits)`` or ``sigmoid(logits)``; the choice goes by ``s + bias`` (fp32 ``[experts]``, for balance), the
+    weights are ``s`` of the chosen, over their sum with ``renormalize``, times ``scale``.  With ``groups`` the experts are
+    that many equal runs, of which the ``top_groups`` whose ``group_best`` (1 or 2) best choices add up to most are chosen
+    from.  Best first, equal choices by their index; values that 32 bits do not tell apart are decided in 64.  A
+    logit of ``-inf`` masks an expert: it comes after all others, with weight 0.  A NaN logit makes the token's weights
+    NaN."""
+
+    del status  # every input is valid on the device
+    if logits.ndim != 2 or logits.dtype not in _lib.DTYPE_CODES or not logits.is_cuda:
+        raise ValueError("route_experts takes CUDA logits [tokens, experts] in bf16, fp16 or fp32")
+    if scores not in SCORES:
+        raise ValueError(f"unknown scores {scores!r}: one of {', '.join(SCORES)}")
+    tokens, experts = (int(v) for v in logits.shape)
+    if experts > 1 and logits.stride(1) != 1 or tokens > 1 and logits.stride(0) < experts:
+        raise ValueError(f"logits need dense rows that do not overlap, not strides {list(logits.stride())}")
+    if bias is not None and (bias.dtype is not torch.float32 or tuple(bias.shape) != (experts,) or
+                             not bias.is_contiguous() or bias.device != logits.device):
+        raise ValueError(f"bias must be dense fp32 [{experts}] on the logits' device")
+    if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
+        raise ValueError("route_experts has no gradient")
+    device, top_k = logits.device, int(top_k)
+    ids = torch.empty(tokens, max(top_k, 0), dtype=torch.int32, device=device)
+    weights = torch.empty(tokens, max(top_k, 0), dtype=torch.float32, device=device)
+    if tokens == 0:
+        return ids, weights
+    with _lib.on_device(device):
+        _lib.check(_lib.load().mie_route_experts(
+            _lib.ptr(logits), row_stride(logits), _lib.DTYPE_CODES[logits.dtype], _lib.ptr(bias), SCORES[scores], tokens,
+            experts, top_k, groups, top_groups, group_best, int(renormalize), float(scale), _lib.ptr(ids),
+            _lib.ptr(weights), _lib.stream_arg(device)))
+    return ids, weights
+
+
+def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, *,
+               activation: str = "silu", residual: torch.Tensor | None = None, status: torch.Tensor) -> torch.Tensor:
+    """``residual + sum_j weights[:, j] down_e (act(gate_e x) * (up_e x))``, ``e = ids[:, j]``, of bf16 rows ``x [tokens,
+    width]``.
+
+    ``gate_up [experts, 2 ff, width]`` holds an expert's gates and then its ups, ``down [experts, width, ff]``; ``ids``
+    (int32 or int64) and ``weights`` (fp32) are ``[tokens, top_k]``, as ``route_experts`` gives them.  An id of -1 is no
+    expert (padding rows); another outside the pool is skipped and reported through ``status``.  An expert may be named
+    twice by a token."""
+
+    if x.ndim != 2 or gate_up.ndim != 3 or down.ndim != 3 or ids.ndim != 2:
+        raise ValueError("expert_mlp takes x [tokens, width], ids [tokens, top_k], gate_up [experts, 2 ff, width] and "
+                         "down [experts, width, ff]")
+    code, device = activation_code(activation), x.device
+    (tokens, width), (experts, double_ff, _), top_k = x.shape, gate_up.shape, int(ids.shape[1])
+    ff = double_ff // 2
+    check_rows("x", x, (tokens, width), device)
+    check_rows("gate_up", gate_up, (experts, 2 * ff, width), device)
+    check_rows("down", down, (experts, width, ff), device)
+    if residual is not None:
+        check_rows("residual", residual, (tokens, width), device)
+    if ids.dtype not in (torch.int32, torch.int64) or ids.shape[0] != tokens or ids.device != device:
+        raise ValueError(f"ids must be int32 or int64 [{tokens}, top_k] on the device of x")
+    if weights.dtype is not torch.float32 or weights.shape != ids.shape or weights.device != device or \
+            not weights.is_contiguous():
+        raise ValueError(f"weights must be dense fp32 {list(ids.shape)} on the device of x")
+    if weights.requires_grad and torch.is_grad_enabled():
+        raise ValueError("weights requires a gradient: this operator has none")
+    lib = _lib.load()
+    out = torch.empty(tokens, width, dtype=torch.bfloat16, device=device)
+    if tokens == 0:
+        return out
+    with _lib.on_device(device):
+        scratch = torch.empty(max(1, lib.mie_expert_scratch_bytes(tokens, top_k, experts, width, ff)), dtype=torch.uint8,
+                              device=device)
+        _lib.check(lib.mie_expert_mlp(
+            _lib.ptr(x), row_stride(x), _lib.index_arg(ids), _lib.ptr(weights), _lib.ptr(gate_up), row_stride(gate_up, 1),
+            row_stride(gate_up), _lib.ptr(down), row_stride(down, 1), row_stride(down), _lib.ptr(residual),
+            0 if residual is None else row_stride(residual), _lib.ptr(out), width, tokens, top_k, experts, width, ff, code,
+            _lib.ptr(scratch), scratch.numel(), _lib.ptr(status), _lib.stream_arg(device)))
+    return out
+
+
+__all__ = ["MAX_EXPERTS", "MAX_TOP_K", "SCORES", "expert_mlp", "route_experts"]

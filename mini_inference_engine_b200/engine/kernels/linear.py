@@ -1,6 +1,10 @@
-"""bf16 projections of decode-sized batches (``csrc/linear.cu``); everything else goes to the library product."""
+"""bf16 projections: of decode-sized batches (``linear``, ``csrc/linear.cu``; everything else goes to the library product),
+and of any number of rows with bias, activation or gate, and residual in the epilogue (``fused_linear``,
+``csrc/fused_linear.cu``)."""
 
 from __future__ import annotations
+
+import math
 
 import torch
 
@@ -56,4 +60,71 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     return out
 
 
-__all__ = ["MAX_ROWS", "linear", "linear_supported", "prefers_own_kernel"]
+ACTIVATIONS = {"none": 0, "silu": 1, "gelu": 2, "relu": 3}  # MIE_ACT_*; gelu is its tanh form
+
+
+def activation_code(name: str | None) -> int:
+    code = ACTIVATIONS.get("none" if name is None else name)
+    if code is None:
+        raise ValueError(f"unknown activation {name!r}: one of {', '.join(ACTIVATIONS)}")
+    return code
+
+
+def check_rows(name: str, tensor: torch.Tensor, shape: tuple[int, ...], device: torch.device) -> None:
+    """A bf16 CUDA tensor of ``shape`` whose rows are dense and do not overlap, and that autograd does not follow."""
+
+    if tensor.dtype is not torch.bfloat16 or tuple(tensor.shape) != shape:
+        raise ValueError(f"{name} must be bf16 {list(shape)}, not {tensor.dtype} {list(tensor.shape)}")
+    if tensor.device != device or device.type != "cuda":
+        raise ValueError(f"{name} must be on the CUDA device of the other operands, not {tensor.device}")
+    if tensor.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient: this operator has none")
+    dense, extent = shape[-1] == 1 or tensor.stride(-1) == 1, shape[-1]
+    for size, stride in zip(shape[-2::-1], tensor.stride()[-2::-1]):
+        if size > 1:
+            dense, extent = dense and stride >= extent, stride * size
+    if not dense:
+        raise ValueError(f"{name} needs rows that are dense and do not overlap, not strides {list(tensor.stride())}")
+
+
+def row_stride(tensor: torch.Tensor, dim: int = 0) -> int:
+    """Stride of a dimension of dense rows; where it has a single entry, that of rows without gaps."""
+
+    return tensor.stride(dim) if tensor.shape[dim] > 1 else math.prod(tensor.shape[dim + 1:])
+
+
+def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
+                 activation: str | None = None, gated: bool = False, residual: torch.Tensor | None = None,
+                 status: torch.Tensor) -> torch.Tensor:
+    """``act(x weight^T + bias) + residual`` in one launch, for ``x [rows, k]`` and ``weight [n, k]``; with ``gated``,
+    ``weight`` and ``bias`` have ``2 n`` rows, gates first, and the result is
+    ``act(x gates^T + bias_g) * (x ups^T + bias_u) + residual``.  bf16 with fp32 sums, rounded once."""
+
+    if x.ndim != 2 or weight.ndim != 2:
+        raise ValueError("fused_linear takes rows [rows, k] and a weight [n, k]")
+    code, device = activation_code(activation), x.device
+    (rows, k), n = x.shape, int(weight.shape[0])
+    check_rows("x", x, (rows, k), device)
+    check_rows("weight", weight, (n, k), device)
+    if gated:
+        if n % 2:
+            raise ValueError(f"a gated weight has as many gates as ups, not {n} rows")
+        n //= 2
+    if n < 1 or k < 1:
+        raise ValueError("fused_linear needs at least one column and one weight row")
+    if bias is not None:
+        check_rows("bias", bias, (2 * n if gated else n,), device)
+    if residual is not None:
+        check_rows("residual", residual, (rows, n), device)
+    out = torch.empty(rows, n, dtype=torch.bfloat16, device=device)
+    if rows == 0:
+        return out
+    with _lib.on_device(device):
+        _lib.check(_lib.load().mie_fused_linear(
+            _lib.ptr(x), row_stride(x), _lib.ptr(weight), row_stride(weight), _lib.ptr(bias), _lib.ptr(residual),
+            0 if residual is None else row_stride(residual), _lib.ptr(out), n, rows, n, k, code, int(gated),
+            _lib.ptr(status), _lib.stream_arg(device)))
+    return out
+
+
+__all__ = ["ACTIVATIONS", "MAX_ROWS", "fused_linear", "linear", "linear_supported", "prefers_own_kernel"]

@@ -1,0 +1,72 @@
+"""What routing and the routed feed-forward refuse, without a GPU."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from mini_inference_engine_b200 import _lib, build
+from mini_inference_engine_b200.engine.kernels.experts import expert_mlp, route_experts
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build.build_library()
+    return _lib.load()
+
+
+def test_refusals_of_the_operators():
+    with pytest.raises(ValueError, match="CUDA logits"):
+        route_experts(torch.zeros(2, 8), 2)
+    x, ids, weights = torch.zeros(2, 16).bfloat16(), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, 2)
+    gate_up, down, status = torch.zeros(4, 16, 16).bfloat16(), torch.zeros(4, 16, 8).bfloat16(), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA device"):
+        expert_mlp(x, ids, weights, gate_up, down, status=status)
+    with pytest.raises(ValueError, match="unknown activation"):
+        expert_mlp(x, ids, weights, gate_up, down, activation="swish", status=status)
+    with pytest.raises(ValueError, match="takes x"):
+        expert_mlp(x, ids, weights, gate_up[0], down, status=status)
+    with pytest.raises(ValueError, match="must be bf16"):
+        expert_mlp(x.float(), ids, weights, gate_up, down, status=status)
+
+
+def route(lib, ld=16, dtype=2, scores=0, tokens=0, experts=16, top_k=2, groups=1, top_groups=1, group_best=1, logits=4096):
+    p = ctypes.c_void_p(4096)
+    return lib.mie_route_experts(ctypes.c_void_p(logits), ld, dtype, None, scores, tokens, experts, top_k, groups,
+                                 top_groups, group_best, 1, 1.0, p, p, None)
+
+
+def test_refusals_of_routing(lib):
+    assert route(lib) == 0 and route(lib, groups=4, top_groups=2, group_best=2, top_k=8) == 0
+    for wrong in ({"logits": 0}, {"ld": 15}, {"dtype": 3}, {"scores": 2}, {"tokens": -1}, {"experts": 0},
+                  {"experts": 1025, "ld": 1025}, {"top_k": 0}, {"top_k": 17}, {"top_k": 33, "experts": 64, "ld": 64},
+                  {"groups": 3}, {"groups": 0}, {"groups": 4, "top_groups": 5}, {"groups": 4, "top_groups": 0},
+                  {"groups": 4, "top_groups": 1, "top_k": 5}, {"groups": 64, "experts": 64, "ld": 64},
+                  {"group_best": 3}, {"groups": 16, "top_groups": 4, "group_best": 2}):
+        assert route(lib, **wrong) == -1, wrong
+
+
+def experts_call(lib, **changes):
+    given = {"x": 4096, "ldx": 16, "ids": 4096, "weights": 4096, "gate_up": 4096, "gate_up_row": 16, "down": 4096,
+             "down_row": 8, "residual": None, "ldr": 16, "y": 4096, "ldy": 16, "tokens": 0, "top_k": 2, "experts": 4,
+             "width": 16, "ff": 8, "activation": 1, "scratch": 4096, "scratch_bytes": 1 << 20, **changes}
+    p = lambda name: ctypes.c_void_p(given[name])  # noqa: E731
+    return lib.mie_expert_mlp(
+        p("x"), given["ldx"], _lib.IndexT(given["ids"], 0, 2, 1), p("weights"), p("gate_up"), given["gate_up_row"], 256,
+        p("down"), given["down_row"], 128, p("residual"), given["ldr"], p("y"), given["ldy"], given["tokens"],
+        given["top_k"], given["experts"], given["width"], given["ff"], given["activation"], p("scratch"),
+        given["scratch_bytes"], None, None)
+
+
+def test_refusals_of_the_feed_forward(lib):
+    assert experts_call(lib) == 0  # no tokens
+    for wrong in ({"x": None}, {"ids": None}, {"weights": None}, {"gate_up": None}, {"down": None}, {"y": None},
+                  {"scratch": None}, {"ldx": 15}, {"gate_up_row": 15}, {"down_row": 7}, {"ldy": 15},
+                  {"residual": 4096, "ldr": 15}, {"tokens": -1}, {"top_k": 0}, {"top_k": 33}, {"experts": 0},
+                  {"experts": 1025}, {"width": 0}, {"ff": 0}, {"activation": 4}, {"tokens": 100, "scratch_bytes": 64},
+                  {"tokens": 1 << 29}):
+        assert experts_call(lib, **wrong) == -1, wrong
+    assert lib.mie_expert_scratch_bytes(8, 2, 4, 16, 8) > 0
+    assert lib.mie_expert_scratch_bytes(-1, 2, 4, 16, 8) == 0
