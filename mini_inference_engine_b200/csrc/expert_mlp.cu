@@ -9,7 +9,9 @@
 //
 // A pair's order among its expert's rows is whatever the counters gave; every row of a product is computed by itself, so
 // the results do not depend on it.  Ids outside [0, experts) take no part: -1 says "no expert", others also set a status bit.
+#include "product_wide.cuh"
 #include "products.cuh"
+#include "rows.cuh"
 
 namespace mie {
 namespace {
@@ -97,11 +99,14 @@ __global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const PlanPar
   const int first = block_scan_before(total, warp_sums);
   if (e < p.experts) place[e] = first + before;
   if (rank == 0) {
-    const int tiles = (total + p.tile_rows - 1) / p.tile_rows;
+    // As few tiles as hold the expert's rows, about equally long, in multiples of 16.
+    int tiles = (total + p.tile_rows - 1) / p.tile_rows;
+    const int rows = tiles > 0 ? ((total + tiles - 1) / tiles + 15) / 16 * 16 : 16;
+    tiles = (total + rows - 1) / rows;
     const int tile = block_scan_before(tiles, warp_sums);
     for (int i = 0; i < tiles; ++i) {
-      const int left = total - i * p.tile_rows;
-      p.tiles[tile + i] = RowTile{e, first + i * p.tile_rows, left < p.tile_rows ? left : p.tile_rows, 0};
+      const int left = total - i * rows;
+      p.tiles[tile + i] = RowTile{e, first + i * rows, left < rows ? left : rows, 0};
     }
     if (e == kPlanThreads - 1) *p.tile_count = tile + tiles;
   }
@@ -114,7 +119,9 @@ __global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const PlanPar
 }
 
 struct CombineParams {
-  const float* rows;  // [tokens * top_k, width]
+  const void* rows;          // [tokens * top_k, width] fp32, or fp16 with
+  const int8_t* exponents;   // [tokens * top_k, exponent_ld], one per 32 entries: value = entry / 2^exponent
+  int exponent_ld;
   IndexView ids;
   const __nv_bfloat16* residual;
   long long ldr;
@@ -123,8 +130,8 @@ struct CombineParams {
   int tokens, top_k, width, experts;
 };
 
-// Adds in the order of the choices.
-__global__ void __launch_bounds__(256) expert_combine_kernel(const CombineParams p) {
+// The residual and the pairs' rows, added in the order of the choices.
+__global__ void __launch_bounds__(256) expert_combine_any_kernel(const CombineParams p) {
   chain_release();
   chain_wait();
   const long long total = (long long)p.tokens * p.width;
@@ -134,31 +141,105 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const CombineParams
     float sum = p.residual != nullptr ? __bfloat162float(p.residual[t * p.ldr + c]) : 0.f;
     for (int j = 0; j < p.top_k; ++j) {
       const long long e = p.ids.at(t, j);
-      if (e >= 0 && e < p.experts) sum += p.rows[(t * p.top_k + j) * p.width + c];
+      if (e >= 0 && e < p.experts) sum += reinterpret_cast<const float*>(p.rows)[(t * p.top_k + j) * p.width + c];
     }
     p.y[t * p.ldy + c] = __float2bfloat16_rn(sum);
   }
 }
 
+// Eight entries a thread; bound by HBM.
+__global__ void __launch_bounds__(256) expert_combine_kernel(const CombineParams p) {
+  chain_release();
+  chain_wait();
+  const int per_row = p.width / 8;
+  const long long total = (long long)p.tokens * per_row;
+  const bool vec_y = p.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
+  const bool vec_r = p.ldr % 8 == 0 && (reinterpret_cast<uintptr_t>(p.residual) & 15) == 0;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+    const long long t = i / per_row;
+    const int c = (int)(i - t * per_row) * 8;
+    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (p.residual != nullptr) {
+      const __nv_bfloat16* r = p.residual + t * p.ldr + c;
+      if (vec_r) {
+        Vec<__nv_bfloat16, 8>::load(r, sum);
+      } else {
+#pragma unroll
+        for (int n = 0; n < 8; ++n) sum[n] = __bfloat162float(r[n]);
+      }
+    }
+    for (int j = 0; j < p.top_k; ++j) {
+      const long long e = p.ids.at(t, j), row = t * p.top_k + j;
+      if (e < 0 || e >= p.experts) continue;
+      const uint4 raw = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.rows) + row * p.width + c);
+      const float scale = __uint_as_float((uint32_t)(127 - p.exponents[row * p.exponent_ld + c / 32]) << 23);
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[n]));
+        sum[2 * n] = fmaf(f.x, scale, sum[2 * n]);
+        sum[2 * n + 1] = fmaf(f.y, scale, sum[2 * n + 1]);
+      }
+    }
+    __nv_bfloat16* y = p.y + t * p.ldy + c;
+    if (vec_y) {
+      Vec<__nv_bfloat16, 8>::store(y, sum);
+    } else {
+#pragma unroll
+      for (int n = 0; n < 8; ++n) y[n] = __float2bfloat16_rn(sum[n]);
+    }
+  }
+}
+
 // Where the parts of the scratch begin.
 struct Scratch {
-  long long order, tiles, tile_count, hidden, rows, total;
-  long long max_tiles;
-  Scratch(long long pairs, int experts, int width, int ff, int tile_rows) {
-    auto take = [this](long long bytes) {
-      const long long at = total;
-      total += (bytes + 255) / 256 * 256;
-      return at;
-    };
+  long long order, tiles, tile_count, hidden, exponents, rows, total;
+  Scratch(long long pairs, int experts, int width, int ff) {
     total = 0;
-    max_tiles = pairs / tile_rows + (pairs < experts ? pairs : experts);
     order = take(pairs * 4);
-    tiles = take(max_tiles * (long long)sizeof(RowTile));
+    tiles = take(most_tiles(pairs, experts, kAnyTile) * (long long)sizeof(RowTile));
     tile_count = take(4);
     hidden = take(pairs * ff * 2);
+    exponents = take(pairs * exponent_ld(width));
     rows = take(pairs * width * 4);
   }
+  long long take(long long bytes) {
+    const long long at = total;
+    total += (bytes + 255) / 256 * 256;
+    return at;
+  }
+  // Every expert's rows in tiles of at least half of tile_rows but one.
+  static long long most_tiles(long long pairs, int experts, int tile_rows) {
+    return 2 * (pairs / tile_rows) + (pairs < experts ? pairs : experts);
+  }
+  static int exponent_ld(int width) { return (width + 31) / 32; }
 };
+
+int launch_plan(const PlanParams& plan, cudaStream_t stream) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(plan.pairs > 4096 ? 8 : 1);
+  config.blockDim = dim3(kPlanThreads);
+  config.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = config.gridDim.x;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = chained_launch_enabled() ? 2 : 1;
+  MIE_CUDA(cudaLaunchKernelEx(&config, expert_plan_kernel, plan));
+  MIE_LAUNCH_CHECK("expert_plan_kernel");
+  return MIE_OK;
+}
+
+int launch_any(const Product& p, long long tiles, cudaStream_t stream) {
+  MIE_CUDA(launch_chained(product_any_kernel<true>,
+                          dim3((unsigned)((p.n + kAnyTile - 1) / kAnyTile), (unsigned)(tiles < 65535 ? tiles : 65535)),
+                          dim3(128), 0, stream, p));
+  MIE_LAUNCH_CHECK("product_any_kernel");
+  return MIE_OK;
+}
 
 }  // namespace
 }  // namespace mie
@@ -167,7 +248,7 @@ using namespace mie;
 
 extern "C" int64_t mie_expert_scratch_bytes(int32_t tokens, int32_t top_k, int32_t experts, int32_t width, int32_t ff) {
   if (tokens < 0 || top_k < 1 || experts < 1 || width < 1 || ff < 1) return 0;
-  return Scratch((long long)tokens * top_k, experts, width, ff, kAnyTile).total;
+  return Scratch((long long)tokens * top_k, experts, width, ff).total;
 }
 
 extern "C" int mie_expert_mlp(const void* x, int64_t ldx, mie_index_t ids, const float* weights, const void* gate_up,
@@ -185,28 +266,12 @@ extern "C" int mie_expert_mlp(const void* x, int64_t ldx, mie_index_t ids, const
                 "a row is longer than its stride");
   MIE_CHECK_ARG(activation >= MIE_ACT_NONE && activation <= MIE_ACT_RELU, "unknown activation %d", activation);
   const int pairs = tokens * top_k;
-  const Scratch s(pairs, experts, width, ff, kAnyTile);
+  const Scratch s(pairs, experts, width, ff);
   MIE_CHECK_ARG(scratch_bytes >= s.total, "scratch of %lld bytes, %lld needed", (long long)scratch_bytes, s.total);
+  MIE_CHECK_ARG((reinterpret_cast<uintptr_t>(scratch) & 255) == 0, "scratch must be 256-byte aligned");
   if (tokens == 0) return MIE_OK;
   uint8_t* base = (uint8_t*)scratch;
   int* order = (int*)(base + s.order);
-
-  PlanParams plan{IndexView(ids), pairs, top_k, experts, kAnyTile, order, (RowTile*)(base + s.tiles),
-                  (int*)(base + s.tile_count), status};
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(pairs > 4096 ? 8 : 1);
-  config.blockDim = dim3(kPlanThreads);
-  config.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = config.gridDim.x;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attr;
-  config.numAttrs = chained_launch_enabled() ? 2 : 1;
-  MIE_CUDA(cudaLaunchKernelEx(&config, expert_plan_kernel, plan));
-  MIE_LAUNCH_CHECK("expert_plan_kernel");
 
   Product up = {};
   up.x = (const __nv_bfloat16*)x, up.ldx = ldx;
@@ -214,27 +279,52 @@ extern "C" int mie_expert_mlp(const void* x, int64_t ldx, mie_index_t ids, const
   up.y = base + s.hidden, up.ldy = ff;
   up.m = pairs, up.n = ff, up.k = width;
   up.activation = activation, up.gated = 1, up.status = status;
-  up.tiles = plan.tiles, up.tile_count = plan.tile_count;
+  up.tiles = (RowTile*)(base + s.tiles), up.tile_count = (int*)(base + s.tile_count);
   up.source = order, up.source_divisor = top_k, up.factor = weights;
-  const unsigned tiles = (unsigned)(s.max_tiles < 65535 ? s.max_tiles : 65535);
-  MIE_CUDA(launch_chained(product_any_kernel<true>, dim3((unsigned)((ff + kAnyTile - 1) / kAnyTile), tiles), dim3(128), 0,
-                          stream, up));
-  MIE_LAUNCH_CHECK("product_any_kernel");
 
   Product out = {};
   out.x = (const __nv_bfloat16*)(base + s.hidden), out.ldx = ff;
   out.w = (const __nv_bfloat16*)down, out.ldw = down_row, out.w_expert = down_expert;
-  out.y = base + s.rows, out.ldy = width, out.wide = 1;
+  out.y = base + s.rows, out.ldy = width;
   out.m = pairs, out.n = width, out.k = ff;
   out.status = status;
-  out.tiles = plan.tiles, out.tile_count = plan.tile_count, out.target = order;
-  MIE_CUDA(launch_chained(product_any_kernel<true>, dim3((unsigned)((width + kAnyTile - 1) / kAnyTile), tiles), dim3(128), 0,
-                          stream, out));
-  MIE_LAUNCH_CHECK("product_any_kernel");
+  out.tiles = up.tiles, out.tile_count = up.tile_count, out.target = order;
 
-  const CombineParams combine{(const float*)(base + s.rows), IndexView(ids), (const __nv_bfloat16*)residual, ldr,
-                              (__nv_bfloat16*)y, ldy, tokens, top_k, width, experts};
-  const long long blocks = ((long long)tokens * width + 255) / 256, most = 16ll * sm_count();
+  CombineParams combine{base + s.rows, (const int8_t*)(base + s.exponents), s.exponent_ld(width), IndexView(ids),
+                        (const __nv_bfloat16*)residual, ldr, (__nv_bfloat16*)y, ldy, tokens, top_k, width, experts};
+
+  const bool wide = wide_takes(up) && wide_takes(out) && width % 8 == 0;
+  const int tile_rows = wide ? kWideRows : kAnyTile;
+  const long long tiles = s.most_tiles(pairs, experts, tile_rows);
+  const PlanParams plan{IndexView(ids), pairs, top_k, experts, tile_rows, order, (RowTile*)(base + s.tiles),
+                        (int*)(base + s.tile_count), status};
+  if (int rc = launch_plan(plan, stream)) return rc;
+  if (!wide) {
+    out.wide = 1;
+    if (int rc = launch_any(up, tiles, stream)) return rc;
+    if (int rc = launch_any(out, tiles, stream)) return rc;
+    const long long blocks = ((long long)tokens * width + 255) / 256, most = 16ll * sm_count();
+    MIE_CUDA(launch_chained(expert_combine_any_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream,
+                            combine));
+    MIE_LAUNCH_CHECK("expert_combine_any_kernel");
+    return MIE_OK;
+  }
+  WideParams q = {};
+  CUtensorMap map_w, map_x;
+  q.p = up;
+  q.weight_tiles = (ff + 127) / 128;
+  if (int rc = weight_map(&map_w, up, experts)) return rc;
+  if (int rc = row_map(&map_x, up, tokens, 1)) return rc;
+  if (int rc = launch_wide<Rows::kUp, true>(map_w, map_x, q, tiles * q.weight_tiles, stream)) return rc;
+  q.p = out;
+  q.weight_tiles = (width + 255) / 256;
+  q.x_box = 32;
+  q.exponents = (int8_t*)(base + s.exponents);
+  q.exponent_ld = s.exponent_ld(width);
+  if (int rc = weight_map(&map_w, out, experts)) return rc;
+  if (int rc = row_map(&map_x, out, pairs, q.x_box)) return rc;
+  if (int rc = launch_wide<Rows::kDown, false>(map_w, map_x, q, tiles * q.weight_tiles, stream)) return rc;
+  const long long blocks = ((long long)tokens * (width / 8) + 255) / 256, most = 16ll * sm_count();
   MIE_CUDA(launch_chained(expert_combine_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream,
                           combine));
   MIE_LAUNCH_CHECK("expert_combine_kernel");

@@ -1,5 +1,48 @@
 // Projections with bias, activation or gate, and residual in their epilogue.
+#include "product_wide.cuh"
 #include "products.cuh"
+
+namespace mie {
+namespace {
+
+int launch_any(const Product& p, cudaStream_t stream) {
+  const int row_tiles = (p.m + kAnyTile - 1) / kAnyTile;
+  MIE_CUDA(launch_chained(product_any_kernel<false>,
+                          dim3((unsigned)((p.n + kAnyTile - 1) / kAnyTile), (unsigned)(row_tiles < 65535 ? row_tiles : 65535)),
+                          dim3(128), 0, stream, p));
+  MIE_LAUNCH_CHECK("product_any_kernel");
+  return MIE_OK;
+}
+
+int launch_dense_wide(const Product& p, cudaStream_t stream) {
+  WideParams q = {};
+  q.p = p;
+  const int channels = p.gated ? 128 : 256, pairs = sm_count() / 2;
+  q.weight_tiles = (p.n + channels - 1) / channels;
+  // Rows of a tile: the time is the rounds' number times the rows, below 128 of which the weights' way through shared memory
+  // takes as long.
+  long long best = 0;
+  for (int rows = kWideRows; rows >= 128; rows -= 16) {
+    const long long tiles = (long long)q.weight_tiles * ((p.m + rows - 1) / rows);
+    const long long cost = (tiles + pairs - 1) / pairs * (rows + 16);
+    if (q.tile_rows == 0 || cost < best) {
+      best = cost;
+      q.tile_rows = rows;
+    }
+  }
+  q.row_tiles = (p.m + q.tile_rows - 1) / q.tile_rows;
+  q.band = 8;
+  q.x_box = q.tile_rows / 2;
+  CUtensorMap map_w, map_x;
+  if (int rc = weight_map(&map_w, p, 1)) return rc;
+  if (int rc = row_map(&map_x, p, p.m, q.x_box)) return rc;
+  const long long tiles = (long long)q.row_tiles * q.weight_tiles;
+  return p.gated ? launch_wide<Rows::kDense, true>(map_w, map_x, q, tiles, stream)
+                 : launch_wide<Rows::kDense, false>(map_w, map_x, q, tiles, stream);
+}
+
+}  // namespace
+}  // namespace mie
 
 using namespace mie;
 
@@ -20,10 +63,5 @@ extern "C" int mie_fused_linear(const void* x, int64_t ldx, const void* w, int64
   p.y = y, p.ldy = ldy;
   p.m = m, p.n = n, p.k = k;
   p.activation = activation, p.gated = gated != 0, p.status = status;
-  const int row_tiles = (m + kAnyTile - 1) / kAnyTile;
-  MIE_CUDA(launch_chained(product_any_kernel<false>,
-                          dim3((unsigned)((n + kAnyTile - 1) / kAnyTile), (unsigned)(row_tiles < 65535 ? row_tiles : 65535)),
-                          dim3(128), 0, stream, p));
-  MIE_LAUNCH_CHECK("product_any_kernel");
-  return MIE_OK;
+  return wide_takes(p) ? launch_dense_wide(p, stream) : launch_any(p, stream);
 }

@@ -1,0 +1,530 @@
+// Products of many rows on CTA pairs.
+//
+// A pair (`cta_group::2`) multiplies 256 weight rows, 128 of each CTA, with up to 256 rows of x, half of which each CTA
+// stages: the weight rows are the M of the tensor-memory accumulator, the rows of x its N, so that a tile of few rows (the
+// end of an expert's) takes a multiple of 16 columns' time and not 256.  Two accumulators: the epilogue of a tile runs under
+// the products of the next.  One warp requests operands (128-byte-swizzled TMA tiles, rows of x by `tile::gather4` where
+// they are scattered), one issues the MMAs of the pair, eight finish.
+//
+// Gated weights are staged as runs of 8 gates and 8 ups: the accumulator fragment of a thread (16 x 256b: channels l / 4 and
+// l / 4 + 8 of lane l) then holds a gate and its up.  Finished values go through shared memory, transposed by `stmatrix`, to
+// whole 128- or 256-byte runs of y's rows.
+#pragma once
+
+#include "products.cuh"
+#include "umma.cuh"
+
+namespace mie {
+namespace {
+
+constexpr int kWideStages = 6;
+constexpr int kWideRows = 256;                 // rows of x a tile
+constexpr int kWideStageBytes = 32 * 1024;     // 128 weight rows and up to 128 rows of x, 64 columns
+constexpr int kWideFinishers = 8;              // warps
+constexpr int kWideThreads = (kWideFinishers + 2) * 32;
+constexpr int kChunk = 32;                     // rows of x that are finished together
+constexpr int kChunkBytes = kChunk * 256;
+constexpr int kWideSmem = kWideStages * kWideStageBytes + 4 * kChunkBytes + 4 * kChunk * 4 + (2 * kWideStages + 4) * 8 + 16 + 1024;
+static_assert(kWideSmem <= 227 * 1024, "shared memory of an SM");
+
+enum class Rows {
+  kDense,  // y rows as x rows, bias, activation or gate, residual
+  kUp,     // routed, gated: x gathered by pair, hidden rows in sorted order with the pair's weight
+  kDown    // routed: sorted hidden rows, y rows by pair as scaled fp16
+};
+
+struct WideParams {
+  Product p;
+  int row_tiles, tile_rows;  // kDense
+  int weight_tiles, band;
+  int x_box;                 // rows of x a TMA request brings (not gathered)
+  int8_t* exponents;         // kDown: [pairs][exponent_ld], one per 32 channels
+  int exponent_ld;
+};
+
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void tmem_relinquish_pair() {
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t addr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+}
+// Signals the barrier at this address in both CTAs of the pair.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                   smem_u32(bar)),
+               "h"((uint16_t)3)
+               : "memory");
+}
+__device__ __forceinline__ void umma_f16_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      :
+      : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t at_rank(const void* local, uint32_t rank) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(local)), "r"(rank));
+  return remote;
+}
+__device__ __forceinline__ void mbar_arrive_at(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// TMA loads of this GPU's memory into this CTA, completing on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_pair_2d(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void tma_pair_3d(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void tma_pair_5d(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3,
+                                            int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5, "
+      "%6, %7}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+      : "memory");
+}
+// Four rows of 128 bytes.
+__device__ __forceinline__ void tma_pair_gather4(void* dst, const CUtensorMap* map, uint32_t bar, int c0, const int (&r)[4]) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, "
+      "%4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(bar), "r"(c0), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+      : "memory");
+}
+// 16 lanes x 32 columns: lane l gets, for every run of 8 columns, columns 2 (l % 4) and + 1 of lanes l / 4 and l / 4 + 8.
+__device__ __forceinline__ void tmem_ld_fragments(uint32_t addr, float (&v)[16]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
+               "r"(d)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) { return Mma16816<__nv_bfloat16>::pack(lo, hi); }
+
+// Tile `index` of the launch.
+struct WideTile {
+  int expert, first, count, weight;
+};
+template <Rows kRows>
+__device__ __forceinline__ WideTile wide_tile(const WideParams& q, int index) {
+  if constexpr (kRows == Rows::kDense) {
+    // Bands of row tiles go through all weights: what runs at one time shares both in L2.
+    const int per_band = q.band * q.weight_tiles, band = index / per_band, in_band = index - band * per_band;
+    const int wide = q.row_tiles - band * q.band < q.band ? q.row_tiles - band * q.band : q.band;
+    const int weight = in_band / wide, row = band * q.band + in_band - weight * wide;
+    const int first = row * q.tile_rows, left = q.p.m - first;
+    return {0, first, left < q.tile_rows ? left : q.tile_rows, weight};
+  } else {
+    const int tile = index / q.weight_tiles;
+    const RowTile t = q.p.tiles[tile];
+    return {t.expert, t.first, t.count, index - tile * q.weight_tiles};
+  }
+}
+
+template <Rows kRows, bool kGated>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
+    product_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const WideParams q) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* chunks = ring + kWideStages * kWideStageBytes;  // [2 groups][2][kChunk][256]
+  int8_t* chunk_exponents = reinterpret_cast<int8_t*>(chunks + 4 * kChunkBytes);  // [2][2][kChunk][4]
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(chunks + 4 * kChunkBytes + 4 * kChunk * 4);  // the first CTA's is used
+  uint64_t* empty_bar = full_bar + kWideStages;
+  uint64_t* acc_full = empty_bar + kWideStages;
+  uint64_t* acc_empty = acc_full + 2;  // the first CTA's is used
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  const Product& p = q.p;
+  const int warp = uniform_warp_index(), lane = threadIdx.x & 31;
+  const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int blocks = (p.k + 63) / 64;
+
+  if (warp == kWideFinishers && lane == 0) {
+    for (int s = 0; s < kWideStages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], 2 * kWideFinishers);
+    }
+    mbar_fence_init();
+    tma_prefetch_desc(&map_w);
+    tma_prefetch_desc(&map_x);
+  }
+  if (warp == kWideFinishers + 1) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  chain_release();
+  chain_wait();
+  const int tiles = (kRows == Rows::kDense ? q.row_tiles : *p.tile_count) * q.weight_tiles;
+
+  if (warp == kWideFinishers) {
+    int step = 0;
+    bool ok = true;
+    for (int index = pair; index < tiles && ok; index += pairs) {
+      const WideTile t = wide_tile<kRows>(q, index);
+      const int half = (t.count + 15) / 16 * 8;  // rows of x that a CTA stages
+      const int boxes = kRows == Rows::kUp ? 0 : (half + q.x_box - 1) / q.x_box;
+      const uint32_t bytes = 2u * (16384u + 128u * (uint32_t)(kRows == Rows::kUp ? half : boxes * q.x_box));
+      const int first = t.first + rank * half;
+      int source[4];
+      if (kRows == Rows::kUp) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          int row = rank * half + lane * 4 + j;
+          row = row < t.count ? row : t.count - 1;  // padding rows: any
+          source[j] = p.source[t.first + row] / p.source_divisor;
+        }
+      }
+      for (int b = 0; b < blocks; ++b, ++step) {
+        const int s = step % kWideStages;
+        uint8_t* dst = ring + (size_t)s * kWideStageBytes;
+        if (!warp_wait_bounded(&empty_bar[s], ((step / kWideStages) & 1u) ^ 1u)) {
+          raise_status(p.status, MIE_STATUS_WAIT_TIMEOUT);
+          ok = false;
+          break;
+        }
+        const uint32_t bar = at_rank(&full_bar[s], 0);
+        if (lane == 0) {
+          if (rank == 0) mbar_expect_tx(&full_bar[s], bytes);
+          if (kGated)
+            tma_pair_5d(dst, &map_w, bar, b * 64, 0, 0, t.weight * 16 + rank * 8, t.expert);
+          else
+            tma_pair_3d(dst, &map_w, bar, b * 64, t.weight * 256 + rank * 128, t.expert);
+          for (int i = 0; i < boxes; ++i)
+            tma_pair_2d(dst + 16384 + (size_t)i * q.x_box * 128, &map_x, bar, b * 64, first + i * q.x_box);
+        }
+        if (kRows == Rows::kUp && lane * 4 < half) tma_pair_gather4(dst + 16384 + lane * 512, &map_x, bar, b * 64, source);
+        __syncwarp();
+      }
+    }
+    // Every stage is free before this CTA ends: no signal of the other one is still under way to it.
+    for (int i = 0; i < kWideStages && ok; ++i, ++step)
+      ok = step < kWideStages || warp_wait_bounded(&empty_bar[step % kWideStages], ((step / kWideStages) & 1u) ^ 1u);
+  } else if (warp == kWideFinishers + 1) {
+    if (rank == 0) {
+      int step = 0, round = 0;
+      bool ok = true;
+      WideTile next = pair < tiles ? wide_tile<kRows>(q, pair) : WideTile{};
+      for (int index = pair; index < tiles && ok; index += pairs, ++round) {
+        const WideTile t = next;
+        if (index + pairs < tiles) next = wide_tile<kRows>(q, index + pairs);  // read ahead of its use
+        const int acc = round & 1;
+        if (!warp_wait_bounded(&acc_empty[acc], ((round >> 1) & 1u) ^ 1u)) {
+          raise_status(p.status, MIE_STATUS_WAIT_TIMEOUT);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t idesc = instr_desc_bf16(256, (t.count + 15) / 16 * 16, 0, 0);
+        for (int b = 0; b < blocks; ++b, ++step) {
+          const int s = step % kWideStages;
+          if (!warp_wait_bounded(&full_bar[s], (step / kWideStages) & 1u)) {
+            raise_status(p.status, MIE_STATUS_WAIT_TIMEOUT);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t a = smem_u32(ring + (size_t)s * kWideStageBytes);
+            const uint64_t da = smem_desc_k128(a), db = smem_desc_k128(a + 16384);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_f16_pair(tmem + acc * 256, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc, b > 0 || k > 0 ? 1u : 0u);
+            umma_commit_pair(&empty_bar[s]);
+            if (b == blocks - 1) umma_commit_pair(&acc_full[acc]);
+          }
+          __syncwarp();
+        }
+      }
+    }
+  } else {
+    constexpr int kCtaChannels = kGated ? 64 : 128;  // of y
+    constexpr int kRowBytes = kCtaChannels * 2;
+    const int group = warp >> 2, quad = warp & 3, threads_of_group = 128;
+    const int sub = lane >> 2, pick = lane & 3;
+    int round = 0, turn = 0;
+    bool ok = true;  // once a wait ran out nothing is stored, but every barrier is met
+    for (int index = pair; index < tiles; index += pairs, ++round) {
+      const WideTile t = wide_tile<kRows>(q, index);
+      const int acc = round & 1;
+      const int channel0 = t.weight * (2 * kCtaChannels) + rank * kCtaChannels;
+      const int n_chunks = (t.count + kChunk - 1) / kChunk;
+      // Bias of this thread's channels.
+      float bias[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+      if (kRows == Rows::kDense && p.bias != nullptr) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int c = channel0 + (kGated ? quad * 16 + h * 8 + sub : quad * 32 + h * 16 + r * 8 + sub);
+            if (c < p.n) bias[h][r] = __bfloat162float(p.bias[kGated && r ? p.n + c : c]);
+          }
+        }
+      }
+      const bool has_residual = kRows == Rows::kDense && p.residual != nullptr;
+      constexpr int kLanesPerRow = kRowBytes / 16, kRowsPerStep = 128 / kLanesPerRow;
+      const int store_row = (int)(threadIdx.x & 127) / kLanesPerRow, store_part = (int)(threadIdx.x & 127) % kLanesPerRow;
+      const int store_channel = channel0 + store_part * 8;
+      const bool vec_residual = has_residual && p.ldr % 8 == 0 && (reinterpret_cast<uintptr_t>(p.residual) & 15) == 0;
+      uint4 held[kChunk / kRowsPerStep];
+      auto load_residual = [&](int chunk) {
+#pragma unroll
+        for (int i = 0; i < kChunk / kRowsPerStep; ++i) {
+          const int row = chunk * kChunk + i * kRowsPerStep + store_row;
+          held[i] = make_uint4(0, 0, 0, 0);
+          if (row >= t.count || store_channel >= p.n) continue;
+          const __nv_bfloat16* src = p.residual + (long long)(t.first + row) * p.ldr + store_channel;
+          if (vec_residual && store_channel + 8 <= p.n) {
+            held[i] = *reinterpret_cast<const uint4*>(src);
+          } else {
+            uint16_t e[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              e[j] = store_channel + j < p.n ? reinterpret_cast<const uint16_t*>(src)[j] : (uint16_t)0;
+            held[i] = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
+                                 e[6] | (uint32_t)e[7] << 16);
+          }
+        }
+      };
+      if (has_residual && group < n_chunks) load_residual(group);
+      if (ok && !warp_wait_bounded(&acc_full[acc], (round >> 1) & 1u)) {
+        ok = false;
+        raise_status(p.status, MIE_STATUS_WAIT_TIMEOUT);
+      }
+      tc_fence_after();
+      bool released = false;
+      for (int chunk = group; chunk < n_chunks; chunk += 2, ++turn) {
+        const int buffer = group * 2 + (turn & 1);
+        uint8_t* stage = chunks + buffer * kChunkBytes;
+        const uint32_t stage_addr = smem_u32(stage);
+        const int token = chunk * kChunk + lane;  // whose factor and target this lane knows
+        const bool token_in = token < t.count;
+        float factor = 1.f;
+        long long target = t.first + token;
+        if (kRows != Rows::kDense && token_in) {
+          const int pair_index = kRows == Rows::kUp ? p.source[t.first + token] : p.target[t.first + token];
+          if (kRows == Rows::kUp) factor = p.factor[pair_index];
+          if (kRows == Rows::kDown) target = pair_index;
+        }
+        float v[2][16];
+        const uint32_t from = tmem + (uint32_t)(acc * 256 + chunk * kChunk) + ((uint32_t)(quad * 32) << 16);
+        tmem_ld_fragments(from, v[0]);
+        tmem_ld_fragments(from + (16u << 16), v[1]);
+        tmem_ld_wait();
+        if (chunk + 2 >= n_chunks) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_at(at_rank(&acc_empty[acc], 0));
+          released = true;
+        }
+        if (has_residual) {
+#pragma unroll
+          for (int i = 0; i < kChunk / kRowsPerStep; ++i) {
+            const int row = i * kRowsPerStep + store_row;
+            *reinterpret_cast<uint4*>(stage + row * kRowBytes + ((store_part ^ (row & 7)) * 16)) = held[i];
+          }
+          asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(threads_of_group) : "memory");
+          if (chunk + 2 < n_chunks) load_residual(chunk + 2);
+        }
+        // Eight tokens at a time: matrices of 8 channels x 8 tokens, transposed on their way to [token][channel].
+        const int part = lane >> 3, line = lane & 7;
+        if constexpr (kGated) {
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const int row = (i + (part >> 1)) * 8 + line;
+            const uint32_t at = stage_addr + (uint32_t)(row * kRowBytes + (((quad * 2 + (part & 1)) ^ (row & 7)) * 16));
+            uint32_t res[4] = {0, 0, 0, 0}, out[4];
+            if (has_residual) ldmatrix_x4_trans(res[0], res[1], res[2], res[3], at);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              const int h = m & 1, f = 4 * (i + (m >> 1));
+              float y[2];
+#pragma unroll
+              for (int c = 0; c < 2; ++c) y[c] = activate(p.activation, v[h][f + c] + bias[h][0]) * (v[h][f + 2 + c] + bias[h][1]);
+              if (kRows == Rows::kUp) {
+                y[0] *= __shfl_sync(0xffffffffu, factor, (i + (m >> 1)) * 8 + pick * 2);
+                y[1] *= __shfl_sync(0xffffffffu, factor, (i + (m >> 1)) * 8 + pick * 2 + 1);
+              }
+              if (has_residual) {
+                const float2 r = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&res[m]));
+                y[0] += r.x;
+                y[1] += r.y;
+              }
+              out[m] = pack_bf16(y[0], y[1]);
+            }
+            stmatrix_x4_trans(at, out[0], out[1], out[2], out[3]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = i * 8 + line;
+            const uint32_t at = stage_addr + (uint32_t)(row * kRowBytes + (((quad * 4 + part) ^ (row & 7)) * 16));
+            uint32_t out[4];
+            if constexpr (kRows == Rows::kDown) {
+              // fp16 with an exponent per token and 32 channels: its largest finite value comes to lie in [2^14, 2^15).
+              float top[2] = {0.f, 0.f};
+#pragma unroll
+              for (int m = 0; m < 4; ++m) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                  const float a = fabsf(v[m >> 1][4 * i + 2 * (m & 1) + c]);
+                  top[c] = fmaxf(top[c], a < INFINITY ? a : 0.f);
+                }
+              }
+              float scale[2];
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
+                int e = 14 + 127 - (int)(__float_as_uint(top[c]) >> 23);
+                e = top[c] == 0.f ? 0 : e > 126 ? 126 : e;
+                scale[c] = __uint_as_float((uint32_t)(e + 127) << 23);
+                if (sub == 0) chunk_exponents[(buffer * kChunk + i * 8 + pick * 2 + c) * 4 + quad] = (int8_t)e;
+              }
+#pragma unroll
+              for (int m = 0; m < 4; ++m) {
+                const int f = 4 * i + 2 * (m & 1);
+                out[m] = Mma16816<__half>::pack(v[m >> 1][f] * scale[0], v[m >> 1][f + 1] * scale[1]);
+              }
+            } else {
+              uint32_t res[4] = {0, 0, 0, 0};
+              if (has_residual) ldmatrix_x4_trans(res[0], res[1], res[2], res[3], at);
+#pragma unroll
+              for (int m = 0; m < 4; ++m) {
+                const int f = 4 * i + 2 * (m & 1);
+                float y[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) y[c] = activate(p.activation, v[m >> 1][f + c] + bias[m >> 1][m & 1]);
+                if (has_residual) {
+                  const float2 r = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&res[m]));
+                  y[0] += r.x;
+                  y[1] += r.y;
+                }
+                out[m] = pack_bf16(y[0], y[1]);
+              }
+            }
+            stmatrix_x4_trans(at, out[0], out[1], out[2], out[3]);
+          }
+        }
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(threads_of_group) : "memory");
+        // Whole runs of y's rows.  The other buffer takes the next chunk, so that one barrier a chunk is enough.
+        const bool vec = p.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
+#pragma unroll
+        for (int i = 0; i < kChunk / kRowsPerStep; ++i) {
+          const int row = i * kRowsPerStep + store_row;
+          const long long to = __shfl_sync(0xffffffffu, target, row);
+          if (chunk * kChunk + row >= t.count || !ok) continue;
+          const uint4 data = *reinterpret_cast<const uint4*>(stage + row * kRowBytes + ((store_part ^ (row & 7)) * 16));
+          if (store_channel < p.n) {
+            uint16_t* dst = reinterpret_cast<uint16_t*>(p.y) + to * p.ldy + store_channel;
+            if (vec && store_channel + 8 <= p.n) {
+              *reinterpret_cast<uint4*>(dst) = data;
+            } else {
+              const uint32_t w[4] = {data.x, data.y, data.z, data.w};
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (store_channel + j < p.n) dst[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+            }
+          }
+          if (kRows == Rows::kDown && store_part % 4 == 0 && store_channel < p.n)
+            q.exponents[to * q.exponent_ld + store_channel / 32] = chunk_exponents[(buffer * kChunk + row) * 4 + store_part / 4];
+        }
+      }
+      if (!released) {  // a group without a chunk of this tile
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_at(at_rank(&acc_empty[acc], 0));
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // no CTA leaves while its barriers or staged rows may be used by the other
+  if (warp == kWideFinishers + 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+inline bool rows_fit_tma(const void* ptr, long long stride) {
+  return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && stride % 8 == 0;
+}
+
+// Weight rows [experts][rows][k]; gated as runs of 8 gates and 8 ups, `rows` of each.
+inline int weight_map(CUtensorMap* out, const Product& p, int experts) {
+  const uint64_t row = (uint64_t)p.ldw * 2, expert = experts > 1 ? (uint64_t)p.w_expert * 2 : row;
+  if (p.gated) {
+    const uint64_t dims[5] = {(uint64_t)p.k, 8, 2, (uint64_t)p.n / 8, (uint64_t)experts};
+    const uint64_t strides[4] = {row, (uint64_t)p.n * row, 8 * row, expert};
+    const uint32_t box[5] = {64, 8, 2, 8, 1};
+    return cached_operand_map(out, 5, p.w, dims, strides, box);
+  }
+  const uint64_t dims[3] = {(uint64_t)p.k, (uint64_t)p.n, (uint64_t)experts};
+  const uint64_t strides[2] = {row, expert};
+  const uint32_t box[3] = {64, 128, 1};
+  return cached_operand_map(out, 3, p.w, dims, strides, box);
+}
+inline int row_map(CUtensorMap* out, const Product& p, long long rows, int box_rows) {
+  const uint64_t dims[2] = {(uint64_t)p.k, (uint64_t)rows};
+  const uint64_t strides[1] = {(uint64_t)p.ldx * 2};
+  const uint32_t box[2] = {64, (uint32_t)box_rows};
+  return cached_operand_map(out, 2, p.x, dims, strides, box);
+}
+// What the pair kernel's loads ask of the operands.
+inline bool wide_takes(const Product& p) {
+  return p.k % 8 == 0 && rows_fit_tma(p.x, p.ldx) && rows_fit_tma(p.w, p.ldw) && p.w_expert % 8 == 0 &&
+         (!p.gated || p.n % 8 == 0);
+}
+
+template <Rows kRows, bool kGated>
+int launch_wide(const CUtensorMap& map_w, const CUtensorMap& map_x, const WideParams& q, long long most_tiles,
+                cudaStream_t stream) {
+  static bool configured[64] = {false};
+  int dev = 0;
+  MIE_CUDA(cudaGetDevice(&dev));
+  if (dev >= 0 && dev < 64 && !configured[dev]) {
+    MIE_CUDA(cudaFuncSetAttribute(product_wide_kernel<kRows, kGated>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem));
+    configured[dev] = true;
+  }
+  const long long most = sm_count() / 2;
+  MIE_CUDA(launch_chained(product_wide_kernel<kRows, kGated>, dim3((unsigned)(2 * (most_tiles < most ? most_tiles : most))),
+                          dim3(kWideThreads), kWideSmem, stream, map_w, map_x, q));
+  MIE_LAUNCH_CHECK("product_wide_kernel");
+  return MIE_OK;
+}
+
+}  // namespace
+}  // namespace mie
