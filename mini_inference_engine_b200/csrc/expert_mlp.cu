@@ -168,17 +168,29 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const CombineParams
         for (int n = 0; n < 8; ++n) sum[n] = __bfloat162float(r[n]);
       }
     }
-    for (int j = 0; j < p.top_k; ++j) {
-      const long long e = p.ids.at(t, j), row = t * p.top_k + j;
-      if (e < 0 || e >= p.experts) continue;
-      const uint4 raw = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.rows) + row * p.width + c);
-      const float scale = __uint_as_float((uint32_t)(127 - p.exponents[row * p.exponent_ld + c / 32]) << 23);
-      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    for (int j0 = 0; j0 < p.top_k; j0 += 4) {  // four pairs' loads in flight
+      uint4 raw[4];
+      float scale[4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[n]));
-        sum[2 * n] = fmaf(f.x, scale, sum[2 * n]);
-        sum[2 * n + 1] = fmaf(f.y, scale, sum[2 * n + 1]);
+      for (int u = 0; u < 4; ++u) {
+        const int j = j0 + u;
+        const long long e = j < p.top_k ? p.ids.at(t, j) : -1, row = t * p.top_k + j;
+        raw[u] = make_uint4(0, 0, 0, 0);
+        scale[u] = 0.f;
+        if (e >= 0 && e < p.experts) {
+          raw[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.rows) + row * p.width + c);
+          scale[u] = __uint_as_float((uint32_t)(127 - p.exponents[row * p.exponent_ld + c / 32]) << 23);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[n]));
+          sum[2 * n] = fmaf(f.x, scale[u], sum[2 * n]);
+          sum[2 * n + 1] = fmaf(f.y, scale[u], sum[2 * n + 1]);
+        }
       }
     }
     __nv_bfloat16* y = p.y + t * p.ldy + c;

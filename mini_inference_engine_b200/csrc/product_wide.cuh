@@ -17,21 +17,25 @@
 namespace mie {
 namespace {
 
-constexpr int kWideStages = 6;
-constexpr int kWideRows = 256;                 // rows of x a tile
-constexpr int kWideStageBytes = 32 * 1024;     // 128 weight rows and up to 128 rows of x, 64 columns
-constexpr int kWideFinishers = 8;              // warps
-constexpr int kWideThreads = (kWideFinishers + 2) * 32;
-constexpr int kChunk = 32;                     // rows of x that are finished together
-constexpr int kChunkBytes = kChunk * 256;
-constexpr int kWideSmem = kWideStages * kWideStageBytes + 4 * kChunkBytes + 4 * kChunk * 4 + (2 * kWideStages + 4) * 8 + 16 + 1024;
-static_assert(kWideSmem <= 227 * 1024, "shared memory of an SM");
-
 enum class Rows {
   kDense,  // y rows as x rows, bias, activation or gate, residual
   kUp,     // routed, gated: x gathered by pair, hidden rows in sorted order with the pair's weight
   kDown    // routed: sorted hidden rows, y rows by pair as scaled fp16
 };
+
+constexpr int kWideStages = 6;
+constexpr int kWideRows = 256;                 // rows of x a tile
+constexpr int kWideStageBytes = 32 * 1024;     // 128 weight rows and up to 128 rows of x, 64 columns
+constexpr int kWideFinishers = 8;              // warps
+constexpr int kGatherers = 8;                  // warps that request gathered rows
+template <Rows kRows>
+constexpr int wide_threads() {
+  return (kWideFinishers + 2 + (kRows == Rows::kUp ? kGatherers : 0)) * 32;
+}
+constexpr int kChunk = 32;                     // rows of x that are finished together
+constexpr int kChunkBytes = kChunk * 256;
+constexpr int kWideSmem = kWideStages * kWideStageBytes + 4 * kChunkBytes + 4 * kChunk * 4 + (2 * kWideStages + 4) * 8 + 16 + 1024;
+static_assert(kWideSmem <= 227 * 1024, "shared memory of an SM");
 
 struct WideParams {
   Product p;
@@ -73,8 +77,9 @@ __device__ __forceinline__ uint32_t at_rank(const void* local, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(local)), "r"(rank));
   return remote;
 }
+// Relaxed: tensor memory has been read when this is reached, and a release would wait for the rows stored before.
 __device__ __forceinline__ void mbar_arrive_at(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // TMA loads of this GPU's memory into this CTA, completing on a barrier of either CTA of the pair.
 __device__ __forceinline__ void tma_pair_2d(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
@@ -100,11 +105,11 @@ __device__ __forceinline__ void tma_pair_5d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 // Four rows of 128 bytes.
-__device__ __forceinline__ void tma_pair_gather4(void* dst, const CUtensorMap* map, uint32_t bar, int c0, const int (&r)[4]) {
+__device__ __forceinline__ void tma_pair_gather4(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int4 r) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, "
       "%4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(map), "r"(bar), "r"(c0), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+      "l"(map), "r"(bar), "r"(c0), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
       : "memory");
 }
 // 16 lanes x 32 columns: lane l gets, for every run of 8 columns, columns 2 (l % 4) and + 1 of lanes l / 4 and l / 4 + 8.
@@ -145,7 +150,7 @@ __device__ __forceinline__ WideTile wide_tile(const WideParams& q, int index) {
 }
 
 template <Rows kRows, bool kGated>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(), 1)
     product_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const WideParams q) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -190,21 +195,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
   if (warp == kWideFinishers) {
     int step = 0;
     bool ok = true;
+    WideTile next = pair < tiles ? wide_tile<kRows>(q, pair) : WideTile{};
     for (int index = pair; index < tiles && ok; index += pairs) {
-      const WideTile t = wide_tile<kRows>(q, index);
+      const WideTile t = next;
+      if (index + pairs < tiles) next = wide_tile<kRows>(q, index + pairs);  // read ahead of its use
       const int half = (t.count + 15) / 16 * 8;  // rows of x that a CTA stages
       const int boxes = kRows == Rows::kUp ? 0 : (half + q.x_box - 1) / q.x_box;
       const uint32_t bytes = 2u * (16384u + 128u * (uint32_t)(kRows == Rows::kUp ? half : boxes * q.x_box));
       const int first = t.first + rank * half;
-      int source[4];
-      if (kRows == Rows::kUp) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          int row = rank * half + lane * 4 + j;
-          row = row < t.count ? row : t.count - 1;  // padding rows: any
-          source[j] = p.source[t.first + row] / p.source_divisor;
-        }
-      }
       for (int b = 0; b < blocks; ++b, ++step) {
         const int s = step % kWideStages;
         uint8_t* dst = ring + (size_t)s * kWideStageBytes;
@@ -213,8 +211,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
           ok = false;
           break;
         }
-        const uint32_t bar = at_rank(&full_bar[s], 0);
-        if (lane == 0) {
+        if (elect_one()) {
+          const uint32_t bar = at_rank(&full_bar[s], 0);
           if (rank == 0) mbar_expect_tx(&full_bar[s], bytes);
           if (kGated)
             tma_pair_5d(dst, &map_w, bar, b * 64, 0, 0, t.weight * 16 + rank * 8, t.expert);
@@ -223,13 +221,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
           for (int i = 0; i < boxes; ++i)
             tma_pair_2d(dst + 16384 + (size_t)i * q.x_box * 128, &map_x, bar, b * 64, first + i * q.x_box);
         }
-        if (kRows == Rows::kUp && lane * 4 < half) tma_pair_gather4(dst + 16384 + lane * 512, &map_x, bar, b * 64, source);
         __syncwarp();
       }
     }
     // Every stage is free before this CTA ends: no signal of the other one is still under way to it.
     for (int i = 0; i < kWideStages && ok; ++i, ++step)
       ok = step < kWideStages || warp_wait_bounded(&empty_bar[step % kWideStages], ((step / kWideStages) & 1u) ^ 1u);
+  } else if (kRows == Rows::kUp && warp > kWideFinishers + 1) {
+    // Rows of x by fours: one request costs its warp about 75 clocks, so that several warps share a stage's 32.
+    constexpr int kFours = 32 / kGatherers;
+    const int gatherer = warp - kWideFinishers - 2;
+    int step = 0, source = 0;
+    bool ok = true;
+    WideTile next = {};
+    auto look_ahead = [&](int index) {  // the next tile and its rows, ahead of their use
+      if (index >= tiles) return;
+      next = wide_tile<kRows>(q, index);
+      int row = rank * ((next.count + 15) / 16 * 8) + (lane / 4 * kGatherers + gatherer) * 4 + lane % 4;
+      row = row < next.count ? row : next.count - 1;  // padding rows: any
+      source = p.source[next.first + row];
+    };
+    look_ahead(pair);
+    for (int index = pair; index < tiles && ok; index += pairs) {
+      const int half = (next.count + 15) / 16 * 8;
+      const int mine = (half / 4 - gatherer + kGatherers - 1) / kGatherers;  // fours of this warp
+      const int row = source / p.source_divisor;
+      int4 fours[kFours];
+#pragma unroll
+      for (int i = 0; i < kFours; ++i)
+        fours[i] = make_int4(__shfl_sync(0xffffffffu, row, 4 * i), __shfl_sync(0xffffffffu, row, 4 * i + 1),
+                             __shfl_sync(0xffffffffu, row, 4 * i + 2), __shfl_sync(0xffffffffu, row, 4 * i + 3));
+      look_ahead(index + pairs);
+      for (int b = 0; b < blocks; ++b, ++step) {
+        const int s = step % kWideStages;
+        if (!warp_wait_bounded(&empty_bar[s], ((step / kWideStages) & 1u) ^ 1u)) {
+          raise_status(p.status, MIE_STATUS_WAIT_TIMEOUT);
+          ok = false;
+          break;
+        }
+        if (elect_one()) {
+          const uint32_t bar = at_rank(&full_bar[s], 0);
+          uint8_t* dst = ring + (size_t)s * kWideStageBytes + 16384 + gatherer * 512;
+#pragma unroll
+          for (int i = 0; i < kFours; ++i)
+            if (i < mine) tma_pair_gather4(dst + i * (kGatherers * 512), &map_x, bar, b * 64, fours[i]);
+        }
+        __syncwarp();
+      }
+    }
   } else if (warp == kWideFinishers + 1) {
     if (rank == 0) {
       int step = 0, round = 0;
@@ -294,6 +333,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
       constexpr int kLanesPerRow = kRowBytes / 16, kRowsPerStep = 128 / kLanesPerRow;
       const int store_row = (int)(threadIdx.x & 127) / kLanesPerRow, store_part = (int)(threadIdx.x & 127) % kLanesPerRow;
       const int store_channel = channel0 + store_part * 8;
+      const bool vec_store = p.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && store_channel + 8 <= p.n;
       const bool vec_residual = has_residual && p.ldr % 8 == 0 && (reinterpret_cast<uintptr_t>(p.residual) & 15) == 0;
       uint4 held[kChunk / kRowsPerStep];
       auto load_residual = [&](int chunk) {
@@ -316,25 +356,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
         }
       };
       if (has_residual && group < n_chunks) load_residual(group);
+      // Row of y and factor of the row that this lane knows of each of the group's chunks: read here, not between the stores.
+      int targets[kWideRows / kChunk / 2];
+      float factors[kWideRows / kChunk / 2];
+#pragma unroll
+      for (int i = 0; i < kWideRows / kChunk / 2; ++i) {
+        const int row = (group + 2 * i) * kChunk + lane;
+        targets[i] = t.first + row;
+        if (kRows == Rows::kDown && row < t.count) targets[i] = p.target[t.first + row];
+        if (kRows == Rows::kUp) factors[i] = row < t.count ? p.factor[p.source[t.first + row]] : 0.f;
+      }
       if (ok && !warp_wait_bounded(&acc_full[acc], (round >> 1) & 1u)) {
         ok = false;
         raise_status(p.status, MIE_STATUS_WAIT_TIMEOUT);
       }
       tc_fence_after();
       bool released = false;
-      for (int chunk = group; chunk < n_chunks; chunk += 2, ++turn) {
+#pragma unroll
+      for (int mine = 0; mine < kWideRows / kChunk / 2; ++mine) {
+        const int chunk = group + 2 * mine;
+        if (chunk >= n_chunks) break;
+        ++turn;
+        const int target = targets[mine];
+        const float factor = kRows == Rows::kUp ? factors[mine] : 1.f;
         const int buffer = group * 2 + (turn & 1);
         uint8_t* stage = chunks + buffer * kChunkBytes;
         const uint32_t stage_addr = smem_u32(stage);
-        const int token = chunk * kChunk + lane;  // whose factor and target this lane knows
-        const bool token_in = token < t.count;
-        float factor = 1.f;
-        long long target = t.first + token;
-        if (kRows != Rows::kDense && token_in) {
-          const int pair_index = kRows == Rows::kUp ? p.source[t.first + token] : p.target[t.first + token];
-          if (kRows == Rows::kUp) factor = p.factor[pair_index];
-          if (kRows == Rows::kDown) target = pair_index;
-        }
         float v[2][16];
         const uint32_t from = tmem + (uint32_t)(acc * 256 + chunk * kChunk) + ((uint32_t)(quad * 32) << 16);
         tmem_ld_fragments(from, v[0]);
@@ -358,105 +405,154 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
         // Eight tokens at a time: matrices of 8 channels x 8 tokens, transposed on their way to [token][channel].
         const int part = lane >> 3, line = lane & 7;
         if constexpr (kGated) {
+          float y[16];  // [8 tokens][h][2]
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              y[4 * i + 2 * h] = v[h][4 * i] + bias[h][0];
+              y[4 * i + 2 * h + 1] = v[h][4 * i + 1] + bias[h][0];
+            }
+          }
+          activate_all(p.activation, y);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float f0 = kRows == Rows::kUp ? __shfl_sync(0xffffffffu, factor, i * 8 + pick * 2) : 1.f;
+            const float f1 = kRows == Rows::kUp ? __shfl_sync(0xffffffffu, factor, i * 8 + pick * 2 + 1) : 1.f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              y[4 * i + 2 * h] *= v[h][4 * i + 2] + bias[h][1];
+              y[4 * i + 2 * h + 1] *= v[h][4 * i + 3] + bias[h][1];
+              if (kRows == Rows::kUp) {
+                y[4 * i + 2 * h] *= f0;
+                y[4 * i + 2 * h + 1] *= f1;
+              }
+            }
+          }
 #pragma unroll
           for (int i = 0; i < 4; i += 2) {
             const int row = (i + (part >> 1)) * 8 + line;
             const uint32_t at = stage_addr + (uint32_t)(row * kRowBytes + (((quad * 2 + (part & 1)) ^ (row & 7)) * 16));
-            uint32_t res[4] = {0, 0, 0, 0}, out[4];
-            if (has_residual) ldmatrix_x4_trans(res[0], res[1], res[2], res[3], at);
+            if (has_residual) {
+              uint32_t res[4];
+              ldmatrix_x4_trans(res[0], res[1], res[2], res[3], at);
+#pragma unroll
+              for (int m = 0; m < 4; ++m) {
+                const float2 r = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&res[m]));
+                y[4 * i + 2 * m] += r.x;
+                y[4 * i + 2 * m + 1] += r.y;
+              }
+            }
+            stmatrix_x4_trans(at, pack_bf16(y[4 * i], y[4 * i + 1]), pack_bf16(y[4 * i + 2], y[4 * i + 3]),
+                              pack_bf16(y[4 * i + 4], y[4 * i + 5]), pack_bf16(y[4 * i + 6], y[4 * i + 7]));
+          }
+        } else if constexpr (kRows == Rows::kDown) {
+          // fp16 with an exponent per token and 32 channels: its largest finite value comes to lie in [2^14, 2^15).  Of the
+          // largest only the exponent is needed, two tokens' to a word.
+          uint32_t top[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float a[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+              a[c] = fmaxf(fmaxf(fabsf(v[0][4 * i + c]), fabsf(v[0][4 * i + 2 + c])),
+                           fmaxf(fabsf(v[1][4 * i + c]), fabsf(v[1][4 * i + 2 + c])));
+            top[i] = (__float_as_uint(a[0]) >> 23) | (__float_as_uint(a[1]) >> 23 << 16);
+          }
+          bool infinite = false;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) infinite |= (top[i] & 0xffffu) == 255u || (top[i] >> 16) == 255u;
+          if (infinite) {  // by finite values alone
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              top[i] = 0;
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                uint32_t most = 0;
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                  const uint32_t e = __float_as_uint(v[m >> 1][4 * i + 2 * (m & 1) + c]) >> 23 & 255u;
+                  most = e < 255u && e > most ? e : most;
+                }
+                top[i] |= most << (16 * c);
+              }
+            }
+          }
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top[i] = __vmaxu2(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // 2^(141 - e) as long as that is a normal number (e >= 15).
+            const int e0 = max((int)(top[i] & 0xffffu), 15), e1 = max((int)(top[i] >> 16), 15);
+            const float s0 = __uint_as_float((uint32_t)(268 - e0) << 23), s1 = __uint_as_float((uint32_t)(268 - e1) << 23);
+            if (sub == 0) {
+              const int at = (buffer * kChunk + i * 8 + pick * 2) * 4 + quad;
+              chunk_exponents[at] = (int8_t)(141 - e0);
+              chunk_exponents[at + 4] = (int8_t)(141 - e1);
+            }
+            uint32_t out[4];
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
-              const int h = m & 1, f = 4 * (i + (m >> 1));
-              float y[2];
-#pragma unroll
-              for (int c = 0; c < 2; ++c) y[c] = activate(p.activation, v[h][f + c] + bias[h][0]) * (v[h][f + 2 + c] + bias[h][1]);
-              if (kRows == Rows::kUp) {
-                y[0] *= __shfl_sync(0xffffffffu, factor, (i + (m >> 1)) * 8 + pick * 2);
-                y[1] *= __shfl_sync(0xffffffffu, factor, (i + (m >> 1)) * 8 + pick * 2 + 1);
-              }
-              if (has_residual) {
-                const float2 r = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&res[m]));
-                y[0] += r.x;
-                y[1] += r.y;
-              }
-              out[m] = pack_bf16(y[0], y[1]);
+              const int f = 4 * i + 2 * (m & 1);
+              out[m] = Mma16816<__half>::pack(v[m >> 1][f] * s0, v[m >> 1][f + 1] * s1);
             }
-            stmatrix_x4_trans(at, out[0], out[1], out[2], out[3]);
+            const int row = i * 8 + line;
+            stmatrix_x4_trans(stage_addr + (uint32_t)(row * kRowBytes + (((quad * 4 + part) ^ (row & 7)) * 16)), out[0], out[1],
+                              out[2], out[3]);
           }
         } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int f = 0; f < 16; ++f) v[h][f] += bias[h][(f >> 1) & 1];
+            activate_all(p.activation, v[h]);
+          }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int row = i * 8 + line;
             const uint32_t at = stage_addr + (uint32_t)(row * kRowBytes + (((quad * 4 + part) ^ (row & 7)) * 16));
-            uint32_t out[4];
-            if constexpr (kRows == Rows::kDown) {
-              // fp16 with an exponent per token and 32 channels: its largest finite value comes to lie in [2^14, 2^15).
-              float top[2] = {0.f, 0.f};
+            if (has_residual) {
+              uint32_t res[4];
+              ldmatrix_x4_trans(res[0], res[1], res[2], res[3], at);
 #pragma unroll
               for (int m = 0; m < 4; ++m) {
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                  const float a = fabsf(v[m >> 1][4 * i + 2 * (m & 1) + c]);
-                  top[c] = fmaxf(top[c], a < INFINITY ? a : 0.f);
-                }
-              }
-              float scale[2];
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-#pragma unroll
-                for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
-                int e = 14 + 127 - (int)(__float_as_uint(top[c]) >> 23);
-                e = top[c] == 0.f ? 0 : e > 126 ? 126 : e;
-                scale[c] = __uint_as_float((uint32_t)(e + 127) << 23);
-                if (sub == 0) chunk_exponents[(buffer * kChunk + i * 8 + pick * 2 + c) * 4 + quad] = (int8_t)e;
-              }
-#pragma unroll
-              for (int m = 0; m < 4; ++m) {
-                const int f = 4 * i + 2 * (m & 1);
-                out[m] = Mma16816<__half>::pack(v[m >> 1][f] * scale[0], v[m >> 1][f + 1] * scale[1]);
-              }
-            } else {
-              uint32_t res[4] = {0, 0, 0, 0};
-              if (has_residual) ldmatrix_x4_trans(res[0], res[1], res[2], res[3], at);
-#pragma unroll
-              for (int m = 0; m < 4; ++m) {
-                const int f = 4 * i + 2 * (m & 1);
-                float y[2];
-#pragma unroll
-                for (int c = 0; c < 2; ++c) y[c] = activate(p.activation, v[m >> 1][f + c] + bias[m >> 1][m & 1]);
-                if (has_residual) {
-                  const float2 r = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&res[m]));
-                  y[0] += r.x;
-                  y[1] += r.y;
-                }
-                out[m] = pack_bf16(y[0], y[1]);
+                const float2 r = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&res[m]));
+                v[m >> 1][4 * i + 2 * (m & 1)] += r.x;
+                v[m >> 1][4 * i + 2 * (m & 1) + 1] += r.y;
               }
             }
-            stmatrix_x4_trans(at, out[0], out[1], out[2], out[3]);
+            stmatrix_x4_trans(at, pack_bf16(v[0][4 * i], v[0][4 * i + 1]), pack_bf16(v[0][4 * i + 2], v[0][4 * i + 3]),
+                              pack_bf16(v[1][4 * i], v[1][4 * i + 1]), pack_bf16(v[1][4 * i + 2], v[1][4 * i + 3]));
           }
         }
         asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(threads_of_group) : "memory");
         // Whole runs of y's rows.  The other buffer takes the next chunk, so that one barrier a chunk is enough.
-        const bool vec = p.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
+        uint4 data[kChunk / kRowsPerStep];
+        int to[kChunk / kRowsPerStep];  // row of y, -1: none
 #pragma unroll
         for (int i = 0; i < kChunk / kRowsPerStep; ++i) {
           const int row = i * kRowsPerStep + store_row;
-          const long long to = __shfl_sync(0xffffffffu, target, row);
-          if (chunk * kChunk + row >= t.count || !ok) continue;
-          const uint4 data = *reinterpret_cast<const uint4*>(stage + row * kRowBytes + ((store_part ^ (row & 7)) * 16));
-          if (store_channel < p.n) {
-            uint16_t* dst = reinterpret_cast<uint16_t*>(p.y) + to * p.ldy + store_channel;
-            if (vec && store_channel + 8 <= p.n) {
-              *reinterpret_cast<uint4*>(dst) = data;
-            } else {
-              const uint32_t w[4] = {data.x, data.y, data.z, data.w};
+          data[i] = *reinterpret_cast<const uint4*>(stage + row * kRowBytes + ((store_part ^ (row & 7)) * 16));
+          to[i] = __shfl_sync(0xffffffffu, target, row);
+          if (chunk * kChunk + row >= t.count || !ok || store_channel >= p.n) to[i] = -1;
+        }
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (store_channel + j < p.n) dst[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
-            }
+        for (int i = 0; i < kChunk / kRowsPerStep; ++i) {
+          uint16_t* dst = reinterpret_cast<uint16_t*>(p.y) + to[i] * p.ldy + store_channel;
+          if (vec_store) {
+            if (to[i] >= 0) *reinterpret_cast<uint4*>(dst) = data[i];
+          } else if (to[i] >= 0) {
+            const uint32_t w[4] = {data[i].x, data[i].y, data[i].z, data[i].w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (store_channel + j < p.n) dst[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
           }
-          if (kRows == Rows::kDown && store_part % 4 == 0 && store_channel < p.n)
-            q.exponents[to * q.exponent_ld + store_channel / 32] = chunk_exponents[(buffer * kChunk + row) * 4 + store_part / 4];
+          if (kRows == Rows::kDown && store_part % 4 == 0 && to[i] >= 0)
+            q.exponents[(long long)to[i] * q.exponent_ld + store_channel / 32] =
+                chunk_exponents[(buffer * kChunk + i * kRowsPerStep + store_row) * 4 + store_part / 4];
         }
       }
       if (!released) {  // a group without a chunk of this tile
@@ -521,7 +617,7 @@ int launch_wide(const CUtensorMap& map_w, const CUtensorMap& map_x, const WidePa
   }
   const long long most = sm_count() / 2;
   MIE_CUDA(launch_chained(product_wide_kernel<kRows, kGated>, dim3((unsigned)(2 * (most_tiles < most ? most_tiles : most))),
-                          dim3(kWideThreads), kWideSmem, stream, map_w, map_x, q));
+                          dim3(wide_threads<kRows>()), kWideSmem, stream, map_w, map_x, q));
   MIE_LAUNCH_CHECK("product_wide_kernel");
   return MIE_OK;
 }

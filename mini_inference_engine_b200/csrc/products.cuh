@@ -53,6 +53,36 @@ __device__ __forceinline__ float activate(int kind, float z) {
   return z;
 }
 
+// The activation of N values at once: their exponentials and reciprocals overlap, and one test finds the thread that has a
+// value whose reciprocal would be flushed (value by value the branches cost 190 clocks each in the pair kernel's epilogue).
+template <int N>
+__device__ __forceinline__ void activate_all(int kind, float (&z)[N]) {
+  if (kind == MIE_ACT_SILU || kind == MIE_ACT_GELU) {
+    float d[N], top = 0.f;  // NaN passes the test and comes through the quotient
+    if (kind == MIE_ACT_SILU) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) d[i] = gate_denominator(z[i] * -kLog2e);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        d[i] = gate_denominator(z[i] * fmaf(z[i] * z[i], -2.f * kLog2e * 0.7978845608028654f * 0.044715f,
+                                            -2.f * kLog2e * 0.7978845608028654f));
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmaxf(top, d[i]);
+    if (top <= kGateLimit) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) z[i] = gate_quotient(z[i], d[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) z[i] = activate(kind, z[i]);
+    }
+  } else if (kind == MIE_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = activate(MIE_ACT_RELU, z[i]);
+  }
+}
+
 // Any alignment and size: 64 rows x 64 columns a block, operands by single loads through shared memory, mma.sync.
 constexpr int kAnyTile = 64, kAnyK = 32;
 
