@@ -20,6 +20,7 @@ struct PlanParams {
   IndexView ids;  // [tokens, top_k]
   int pairs, top_k, experts, tile_rows;
   int* order;     // [pairs] sorted row -> pair
+  int* position;  // [pairs] pair -> sorted row, -1 for a pair that takes no part
   RowTile* tiles;
   int* tile_count;
   int* status;
@@ -79,12 +80,20 @@ __global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const PlanPar
   for (int e = threadIdx.x; e < p.experts; e += kPlanThreads) count[e] = 0;
   __syncthreads();
   chain_wait();
-  for (int i = begin + threadIdx.x; i < end; i += kPlanThreads) {
-    const long long e = p.ids.at(i / p.top_k, i % p.top_k);
-    if (e >= 0 && e < p.experts)
-      atomicAdd(&count[e], 1);
-    else if (e != -1)
-      raise_status(p.status, MIE_STATUS_BAD_EXPERT);
+  // A pair's place among its expert's, in this CTA's part, is kept in `position`.
+  for (int i = begin + threadIdx.x; i < end; i += 4 * kPlanThreads) {
+    long long e[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = i + u * kPlanThreads, row = j / p.top_k;
+      e[u] = j < end ? p.ids.at(row, j - row * p.top_k) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const bool valid = e[u] >= 0 && e[u] < p.experts;
+      if (!valid && e[u] != -1) raise_status(p.status, MIE_STATUS_BAD_EXPERT);
+      if (i + u * kPlanThreads < end) p.position[i + u * kPlanThreads] = valid ? atomicAdd(&count[e[u]], 1) : -1;
+    }
   }
   plan_cluster_sync();
   const int e = threadIdx.x;
@@ -111,23 +120,36 @@ __global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const PlanPar
     if (e == kPlanThreads - 1) *p.tile_count = tile + tiles;
   }
   __syncthreads();
-  for (int i = begin + threadIdx.x; i < end; i += kPlanThreads) {
-    const long long expert = p.ids.at(i / p.top_k, i % p.top_k);
-    if (expert >= 0 && expert < p.experts) p.order[atomicAdd(&place[expert], 1)] = i;
+  for (int i = begin + threadIdx.x; i < end; i += 4 * kPlanThreads) {
+    long long expert[4];
+    int within[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = i + u * kPlanThreads, row = j / p.top_k;
+      within[u] = j < end ? p.position[j] : -1;
+      expert[u] = j < end ? p.ids.at(row, j - row * p.top_k) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (within[u] < 0) continue;
+      const int j = i + u * kPlanThreads, sorted = place[expert[u]] + within[u];
+      p.order[sorted] = j;
+      p.position[j] = sorted;
+    }
   }
   plan_cluster_sync();  // no CTA leaves while another may still read its counts
 }
 
 struct CombineParams {
-  const void* rows;          // [tokens * top_k, width] fp32, or fp16 with
-  const int8_t* exponents;   // [tokens * top_k, exponent_ld], one per 32 entries: value = entry / 2^exponent
+  const void* rows;          // [pairs, width] in sorted order: fp32, or fp16 with
+  const int8_t* exponents;   // [pairs, exponent_ld], one per 32 entries: value = entry / 2^exponent
   int exponent_ld;
-  IndexView ids;
+  const int* position;       // [tokens, top_k] sorted row of a pair or -1
   const __nv_bfloat16* residual;
   long long ldr;
   __nv_bfloat16* y;
   long long ldy;
-  int tokens, top_k, width, experts;
+  int tokens, top_k, width;
 };
 
 // The residual and the pairs' rows, added in the order of the choices.
@@ -140,75 +162,74 @@ __global__ void __launch_bounds__(256) expert_combine_any_kernel(const CombinePa
     const int c = (int)(i - t * p.width);
     float sum = p.residual != nullptr ? __bfloat162float(p.residual[t * p.ldr + c]) : 0.f;
     for (int j = 0; j < p.top_k; ++j) {
-      const long long e = p.ids.at(t, j);
-      if (e >= 0 && e < p.experts) sum += reinterpret_cast<const float*>(p.rows)[(t * p.top_k + j) * p.width + c];
+      const long long row = p.position[t * p.top_k + j];
+      if (row >= 0) sum += reinterpret_cast<const float*>(p.rows)[row * p.width + c];
     }
     p.y[t * p.ldy + c] = __float2bfloat16_rn(sum);
   }
 }
 
-// Eight entries a thread; bound by HBM.
+// Eight entries a thread, eight pairs' rows in flight; bound by HBM.
 __global__ void __launch_bounds__(256) expert_combine_kernel(const CombineParams p) {
   chain_release();
-  chain_wait();
-  const int per_row = p.width / 8;
-  const long long total = (long long)p.tokens * per_row;
   const bool vec_y = p.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
   const bool vec_r = p.ldr % 8 == 0 && (reinterpret_cast<uintptr_t>(p.residual) & 15) == 0;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
-    const long long t = i / per_row;
-    const int c = (int)(i - t * per_row) * 8;
-    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (p.residual != nullptr) {
-      const __nv_bfloat16* r = p.residual + t * p.ldr + c;
-      if (vec_r) {
-        Vec<__nv_bfloat16, 8>::load(r, sum);
+  chain_wait();
+  for (long long t = (long long)blockIdx.x * blockDim.y + threadIdx.y; t < p.tokens; t += (long long)gridDim.x * blockDim.y) {
+    for (int c = threadIdx.x * 8; c < p.width; c += blockDim.x * 8) {
+      float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (p.residual != nullptr) {
+        const __nv_bfloat16* r = p.residual + t * p.ldr + c;
+        if (vec_r) {
+          Vec<__nv_bfloat16, 8>::load(r, sum);
+        } else {
+#pragma unroll
+          for (int n = 0; n < 8; ++n) sum[n] = __bfloat162float(r[n]);
+        }
+      }
+      for (int j0 = 0; j0 < p.top_k; j0 += 8) {
+        uint4 raw[8];
+        int exponent[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const long long row = j0 + u < p.top_k ? p.position[t * p.top_k + j0 + u] : -1;
+          raw[u] = make_uint4(0, 0, 0, 0);
+          exponent[u] = 0;
+          if (row >= 0) {
+            raw[u] = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.rows) + row * p.width + c));
+            exponent[u] = p.exponents[row * p.exponent_ld + c / 32];
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float scale = __uint_as_float((uint32_t)(127 - exponent[u]) << 23);
+          const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[n]));
+            sum[2 * n] = fmaf(f.x, scale, sum[2 * n]);
+            sum[2 * n + 1] = fmaf(f.y, scale, sum[2 * n + 1]);
+          }
+        }
+      }
+      __nv_bfloat16* y = p.y + t * p.ldy + c;
+      if (vec_y) {
+        Vec<__nv_bfloat16, 8>::store(y, sum);
       } else {
 #pragma unroll
-        for (int n = 0; n < 8; ++n) sum[n] = __bfloat162float(r[n]);
+        for (int n = 0; n < 8; ++n) y[n] = __float2bfloat16_rn(sum[n]);
       }
-    }
-    for (int j0 = 0; j0 < p.top_k; j0 += 4) {  // four pairs' loads in flight
-      uint4 raw[4];
-      float scale[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int j = j0 + u;
-        const long long e = j < p.top_k ? p.ids.at(t, j) : -1, row = t * p.top_k + j;
-        raw[u] = make_uint4(0, 0, 0, 0);
-        scale[u] = 0.f;
-        if (e >= 0 && e < p.experts) {
-          raw[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.rows) + row * p.width + c);
-          scale[u] = __uint_as_float((uint32_t)(127 - p.exponents[row * p.exponent_ld + c / 32]) << 23);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[n]));
-          sum[2 * n] = fmaf(f.x, scale[u], sum[2 * n]);
-          sum[2 * n + 1] = fmaf(f.y, scale[u], sum[2 * n + 1]);
-        }
-      }
-    }
-    __nv_bfloat16* y = p.y + t * p.ldy + c;
-    if (vec_y) {
-      Vec<__nv_bfloat16, 8>::store(y, sum);
-    } else {
-#pragma unroll
-      for (int n = 0; n < 8; ++n) y[n] = __float2bfloat16_rn(sum[n]);
     }
   }
 }
 
 // Where the parts of the scratch begin.
 struct Scratch {
-  long long order, tiles, tile_count, hidden, exponents, rows, total;
+  long long order, position, tiles, tile_count, hidden, exponents, rows, total;
   Scratch(long long pairs, int experts, int width, int ff) {
     total = 0;
     order = take(pairs * 4);
+    position = take(pairs * 4);
     tiles = take(most_tiles(pairs, experts, kAnyTile) * (long long)sizeof(RowTile));
     tile_count = take(4);
     hidden = take(pairs * ff * 2);
@@ -300,15 +321,15 @@ extern "C" int mie_expert_mlp(const void* x, int64_t ldx, mie_index_t ids, const
   out.y = base + s.rows, out.ldy = width;
   out.m = pairs, out.n = width, out.k = ff;
   out.status = status;
-  out.tiles = up.tiles, out.tile_count = up.tile_count, out.target = order;
+  out.tiles = up.tiles, out.tile_count = up.tile_count;
 
-  CombineParams combine{base + s.rows, (const int8_t*)(base + s.exponents), s.exponent_ld(width), IndexView(ids),
-                        (const __nv_bfloat16*)residual, ldr, (__nv_bfloat16*)y, ldy, tokens, top_k, width, experts};
+  CombineParams combine{base + s.rows, (const int8_t*)(base + s.exponents), s.exponent_ld(width), (const int*)(base + s.position),
+                        (const __nv_bfloat16*)residual, ldr, (__nv_bfloat16*)y, ldy, tokens, top_k, width};
 
-  const bool wide = wide_takes(up) && wide_takes(out) && width % 8 == 0;
+  const bool wide = wide_takes(up) && wide_takes(out) && direct_takes(out);
   const int tile_rows = wide ? kWideRows : kAnyTile;
   const long long tiles = s.most_tiles(pairs, experts, tile_rows);
-  const PlanParams plan{IndexView(ids), pairs, top_k, experts, tile_rows, order, (RowTile*)(base + s.tiles),
+  const PlanParams plan{IndexView(ids), pairs, top_k, experts, tile_rows, order, (int*)(base + s.position), (RowTile*)(base + s.tiles),
                         (int*)(base + s.tile_count), status};
   if (int rc = launch_plan(plan, stream)) return rc;
   if (!wide) {
@@ -322,23 +343,25 @@ extern "C" int mie_expert_mlp(const void* x, int64_t ldx, mie_index_t ids, const
     return MIE_OK;
   }
   WideParams q = {};
-  CUtensorMap map_w, map_x;
+  WeightMaps maps;
+  CUtensorMap map_x;
   q.p = up;
   q.weight_tiles = (ff + 127) / 128;
-  if (int rc = weight_map(&map_w, up, experts)) return rc;
+  if (int rc = weight_maps(&maps, up, experts, false)) return rc;
   if (int rc = row_map(&map_x, up, tokens, 1)) return rc;
-  if (int rc = launch_wide<Rows::kUp, true>(map_w, map_x, q, tiles * q.weight_tiles, stream)) return rc;
+  if (int rc = launch_wide<Rows::kUp, true, false>(maps, map_x, q, tiles * q.weight_tiles, stream)) return rc;
   q.p = out;
   q.weight_tiles = (width + 255) / 256;
   q.x_box = 32;
   q.exponents = (int8_t*)(base + s.exponents);
   q.exponent_ld = s.exponent_ld(width);
-  if (int rc = weight_map(&map_w, out, experts)) return rc;
+  if (int rc = weight_maps(&maps, out, experts, true)) return rc;
   if (int rc = row_map(&map_x, out, pairs, q.x_box)) return rc;
-  if (int rc = launch_wide<Rows::kDown, false>(map_w, map_x, q, tiles * q.weight_tiles, stream)) return rc;
-  const long long blocks = ((long long)tokens * (width / 8) + 255) / 256, most = 16ll * sm_count();
-  MIE_CUDA(launch_chained(expert_combine_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream,
-                          combine));
+  if (int rc = launch_wide<Rows::kDown, false, true>(maps, map_x, q, tiles * q.weight_tiles, stream)) return rc;
+  const int lanes = width / 8 < 256 ? (width / 8 + 31) / 32 * 32 : 256, rows_per_block = 256 / lanes;
+  const long long blocks = ((long long)tokens + rows_per_block - 1) / rows_per_block, most = 16ll * sm_count();
+  MIE_CUDA(launch_chained(expert_combine_kernel, dim3((unsigned)(blocks < most ? blocks : most)),
+                          dim3((unsigned)lanes, (unsigned)rows_per_block), 0, stream, combine));
   MIE_LAUNCH_CHECK("expert_combine_kernel");
   return MIE_OK;
 }

@@ -33,12 +33,15 @@ int launch_dense_wide(const Product& p, cudaStream_t stream) {
   q.row_tiles = (p.m + q.tile_rows - 1) / q.tile_rows;
   q.band = 8;
   q.x_box = q.tile_rows / 2;
-  CUtensorMap map_w, map_x;
-  if (int rc = weight_map(&map_w, p, 1)) return rc;
+  WeightMaps maps;
+  CUtensorMap map_x;
+  const bool direct = direct_takes(p);
+  if (int rc = weight_maps(&maps, p, 1, direct)) return rc;
   if (int rc = row_map(&map_x, p, p.m, q.x_box)) return rc;
   const long long tiles = (long long)q.row_tiles * q.weight_tiles;
-  return p.gated ? launch_wide<Rows::kDense, true>(map_w, map_x, q, tiles, stream)
-                 : launch_wide<Rows::kDense, false>(map_w, map_x, q, tiles, stream);
+  return p.gated  ? launch_wide<Rows::kDense, true, false>(maps, map_x, q, tiles, stream)
+         : direct ? launch_wide<Rows::kDense, false, true>(maps, map_x, q, tiles, stream)
+                  : launch_wide<Rows::kDense, false, false>(maps, map_x, q, tiles, stream);
 }
 
 }  // namespace

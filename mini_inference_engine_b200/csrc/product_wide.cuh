@@ -23,7 +23,11 @@ enum class Rows {
   kDown    // routed: sorted hidden rows, y rows by pair as scaled fp16
 };
 
-constexpr int kWideStages = 6;
+// Finished values go to y straight from the accumulator's fragments (kDirect), or through shared memory.
+template <bool kDirect>
+constexpr int wide_stages() {
+  return kDirect ? 7 : 6;
+}
 constexpr int kWideRows = 256;                 // rows of x a tile
 constexpr int kWideStageBytes = 32 * 1024;     // 128 weight rows and up to 128 rows of x, 64 columns
 constexpr int kWideFinishers = 8;              // warps
@@ -34,8 +38,18 @@ constexpr int wide_threads() {
 }
 constexpr int kChunk = 32;                     // rows of x that are finished together
 constexpr int kChunkBytes = kChunk * 256;
-constexpr int kWideSmem = kWideStages * kWideStageBytes + 4 * kChunkBytes + 4 * kChunk * 4 + (2 * kWideStages + 4) * 8 + 16 + 1024;
-static_assert(kWideSmem <= 227 * 1024, "shared memory of an SM");
+template <bool kDirect>
+constexpr int wide_smem() {
+  return wide_stages<kDirect>() * (kWideStageBytes + 16) + (kDirect ? 0 : 4 * kChunkBytes) + 4 * 8 + 16 + 1024;
+}
+static_assert(wide_smem<false>() <= 227 * 1024 && wide_smem<true>() <= 227 * 1024, "shared memory of an SM");
+
+// A CTA's 128 weight rows as the finishers want them: gated, 8 runs of 8 gates and their 8 ups; direct, 4 runs of 32 in the
+// order 4 s + j -> 8 j + s; otherwise as they are.  `all` brings them at once; where the last run is cut short they come run by
+// run, the whole ones by `run`, the rest of the last one by `rest`.
+struct WeightMaps {
+  CUtensorMap all, run, rest;
+};
 
 struct WideParams {
   Product p;
@@ -149,14 +163,15 @@ __device__ __forceinline__ WideTile wide_tile(const WideParams& q, int index) {
   }
 }
 
-template <Rows kRows, bool kGated>
+template <Rows kRows, bool kGated, bool kDirect>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(), 1)
-    product_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const WideParams q) {
+    product_wide_kernel(const __grid_constant__ WeightMaps maps, const __grid_constant__ CUtensorMap map_x, const WideParams q) {
+  static_assert(!(kGated && kDirect) && (kRows != Rows::kDown || kDirect), "what there are finishers for");
+  constexpr int kWideStages = wide_stages<kDirect>();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t* chunks = ring + kWideStages * kWideStageBytes;  // [2 groups][2][kChunk][256]
-  int8_t* chunk_exponents = reinterpret_cast<int8_t*>(chunks + 4 * kChunkBytes);  // [2][2][kChunk][4]
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(chunks + 4 * kChunkBytes + 4 * kChunk * 4);  // the first CTA's is used
+  uint8_t* chunks = ring + kWideStages * kWideStageBytes;  // [2 groups][2][kChunk][256], not kDirect
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(chunks + (kDirect ? 0 : 4 * kChunkBytes));  // the first CTA's is used
   uint64_t* empty_bar = full_bar + kWideStages;
   uint64_t* acc_full = empty_bar + kWideStages;
   uint64_t* acc_empty = acc_full + 2;  // the first CTA's is used
@@ -176,7 +191,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(
       mbar_init(&acc_empty[a], 2 * kWideFinishers);
     }
     mbar_fence_init();
-    tma_prefetch_desc(&map_w);
+    tma_prefetch_desc(&maps.all);
     tma_prefetch_desc(&map_x);
   }
   if (warp == kWideFinishers + 1) {
@@ -214,10 +229,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(
         if (elect_one()) {
           const uint32_t bar = at_rank(&full_bar[s], 0);
           if (rank == 0) mbar_expect_tx(&full_bar[s], bytes);
-          if (kGated)
-            tma_pair_5d(dst, &map_w, bar, b * 64, 0, 0, t.weight * 16 + rank * 8, t.expert);
-          else
-            tma_pair_3d(dst, &map_w, bar, b * 64, t.weight * 256 + rank * 128, t.expert);
+          if constexpr (kGated || kDirect) {
+            constexpr int kRun = kGated ? 8 : 32, kRuns = kGated ? 8 : 4, kRunBytes = 16384 / kRuns;
+            const int run = (t.weight * 2 + rank) * kRuns, whole = p.n / kRun;
+            if (run + kRuns <= whole || whole * kRun == p.n) {
+              tma_pair_5d(dst, &maps.all, bar, b * 64, 0, 0, run, t.expert);
+            } else {
+              for (int i = 0; i < kRuns; ++i) {
+                if (run + i == whole)
+                  tma_pair_5d(dst + i * kRunBytes, &maps.rest, bar, b * 64, 0, 0, 0, t.expert);
+                else
+                  tma_pair_5d(dst + i * kRunBytes, &maps.run, bar, b * 64, 0, 0, run + i, t.expert);
+              }
+            }
+          } else {
+            tma_pair_3d(dst, &maps.all, bar, b * 64, t.weight * 256 + rank * 128, t.expert);
+          }
           for (int i = 0; i < boxes; ++i)
             tma_pair_2d(dst + 16384 + (size_t)i * q.x_box * 128, &map_x, bar, b * 64, first + i * q.x_box);
         }
@@ -305,6 +332,138 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(
         }
       }
     }
+  } else if constexpr (kDirect) {
+    // The weight rows of a run of 32 are staged in the order 4 s + j -> 8 j + s, so that a thread's four accumulators of a
+    // row of x are neighbours in y: 8 bytes a thread, 64 a row of y and warp, no shared memory (whose bandwidth the MMAs'
+    // operands take: the staged form's loads took 200 clocks each).
+    const int group = warp >> 2, quad = warp & 3, sub = lane >> 2, pick = lane & 3;
+    int round = 0;
+    bool ok = true;  // once a wait ran out nothing is stored
+    for (int index = pair; index < tiles; index += pairs, ++round) {
+      const WideTile t = wide_tile<kRows>(q, index);
+      const int acc = round & 1;
+      const int channel = t.weight * 256 + rank * 128 + quad * 32 + 4 * sub;  // the first of this thread's
+      const int n_chunks = (t.count + kChunk - 1) / kChunk;
+      const bool in = channel < p.n;
+      float bias[4] = {0.f, 0.f, 0.f, 0.f};
+      if (kRows == Rows::kDense && p.bias != nullptr && in) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bias[j] = __bfloat162float(p.bias[channel + j]);
+      }
+      const bool has_residual = kRows == Rows::kDense && p.residual != nullptr;
+      uint2 held[8];  // residual of the next chunk: rows 8 i + 2 pick + c
+      auto load_residual = [&](int chunk) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = chunk * kChunk + (i >> 1) * 8 + 2 * pick + (i & 1);
+          held[i] = make_uint2(0, 0);
+          if (row < t.count && in)
+            held[i] = *reinterpret_cast<const uint2*>(p.residual + (long long)(t.first + row) * p.ldr + channel);
+        }
+      };
+      if (has_residual && group < n_chunks) load_residual(group);
+      if (ok && !warp_wait_bounded(&acc_full[acc], (round >> 1) & 1u)) {
+        ok = false;
+        raise_status(p.status, MIE_STATUS_WAIT_TIMEOUT);
+      }
+      tc_fence_after();
+      for (int chunk = group; chunk < n_chunks; chunk += 2) {
+        float v[2][16];  // [j / 2][4 i + 2 (j % 2) + c]
+        const uint32_t from = tmem + (uint32_t)(acc * 256 + chunk * kChunk) + ((uint32_t)(quad * 32) << 16);
+        tmem_ld_fragments(from, v[0]);
+        tmem_ld_fragments(from + (16u << 16), v[1]);
+        tmem_ld_wait();
+        if (chunk + 2 >= n_chunks) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_at(at_rank(&acc_empty[acc], 0));
+        }
+        const int row0 = chunk * kChunk + 2 * pick;
+        uint16_t* y = reinterpret_cast<uint16_t*>(p.y) + (long long)(t.first + row0) * p.ldy + channel;
+        if constexpr (kRows == Rows::kDown) {
+          // fp16 with an exponent per token and 32 channels: its largest finite value comes to lie in [2^14, 2^15).  Of the
+          // largest only the exponent is needed, two tokens' to a word.
+          uint32_t top[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float a[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+              a[c] = fmaxf(fmaxf(fabsf(v[0][4 * i + c]), fabsf(v[0][4 * i + 2 + c])),
+                           fmaxf(fabsf(v[1][4 * i + c]), fabsf(v[1][4 * i + 2 + c])));
+            top[i] = (__float_as_uint(a[0]) >> 23) | (__float_as_uint(a[1]) >> 23 << 16);
+          }
+          bool infinite = false;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) infinite |= (top[i] & 0xffffu) == 255u || (top[i] >> 16) == 255u;
+          if (infinite) {  // by finite values alone
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              top[i] = 0;
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                uint32_t most = 0;
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                  const uint32_t e = __float_as_uint(v[m >> 1][4 * i + 2 * (m & 1) + c]) >> 23 & 255u;
+                  most = e < 255u && e > most ? e : most;
+                }
+                top[i] |= most << (16 * c);
+              }
+            }
+          }
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top[i] = __vmaxu2(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // 2^(141 - e) as long as that is a normal number (e >= 15).
+            const int e[2] = {max((int)(top[i] & 0xffffu), 15), max((int)(top[i] >> 16), 15)};
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float scale = __uint_as_float((uint32_t)(268 - e[c]) << 23);
+              const uint2 out = make_uint2(Mma16816<__half>::pack(v[0][4 * i + c] * scale, v[0][4 * i + 2 + c] * scale),
+                                           Mma16816<__half>::pack(v[1][4 * i + c] * scale, v[1][4 * i + 2 + c] * scale));
+              if (row0 + 8 * i + c < t.count && in && ok) {
+                *reinterpret_cast<uint2*>(y + (long long)(8 * i + c) * p.ldy) = out;
+                if (sub == 0)
+                  q.exponents[(long long)(t.first + row0 + 8 * i + c) * q.exponent_ld + channel / 32] = (int8_t)(141 - e[c]);
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int f = 0; f < 16; ++f) v[h][f] += bias[2 * h + ((f >> 1) & 1)];
+            activate_all(p.activation, v[h]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float a[4] = {v[0][4 * i + c], v[0][4 * i + 2 + c], v[1][4 * i + c], v[1][4 * i + 2 + c]};
+              if (has_residual) {
+                const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&held[2 * i + c].x));
+                const float2 hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&held[2 * i + c].y));
+                a[0] += lo.x, a[1] += lo.y, a[2] += hi.x, a[3] += hi.y;
+              }
+              if (row0 + 8 * i + c < t.count && in && ok)
+                *reinterpret_cast<uint2*>(y + (long long)(8 * i + c) * p.ldy) =
+                    make_uint2(pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]));
+            }
+          }
+          if (has_residual && chunk + 2 < n_chunks) load_residual(chunk + 2);
+        }
+      }
+      if (group >= n_chunks) {  // no chunk of this tile
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_at(at_rank(&acc_empty[acc], 0));
+      }
+    }
   } else {
     constexpr int kCtaChannels = kGated ? 64 : 128;  // of y
     constexpr int kRowBytes = kCtaChannels * 2;
@@ -356,15 +515,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(
         }
       };
       if (has_residual && group < n_chunks) load_residual(group);
-      // Row of y and factor of the row that this lane knows of each of the group's chunks: read here, not between the stores.
-      int targets[kWideRows / kChunk / 2];
+      // Factor of the row that this lane knows of each of the group's chunks: read here, not between the stores.
       float factors[kWideRows / kChunk / 2];
+      if (kRows == Rows::kUp) {
 #pragma unroll
-      for (int i = 0; i < kWideRows / kChunk / 2; ++i) {
-        const int row = (group + 2 * i) * kChunk + lane;
-        targets[i] = t.first + row;
-        if (kRows == Rows::kDown && row < t.count) targets[i] = p.target[t.first + row];
-        if (kRows == Rows::kUp) factors[i] = row < t.count ? p.factor[p.source[t.first + row]] : 0.f;
+        for (int i = 0; i < kWideRows / kChunk / 2; ++i) {
+          const int row = (group + 2 * i) * kChunk + lane;
+          factors[i] = row < t.count ? p.factor[p.source[t.first + row]] : 0.f;
+        }
       }
       if (ok && !warp_wait_bounded(&acc_full[acc], (round >> 1) & 1u)) {
         ok = false;
@@ -377,7 +535,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(
         const int chunk = group + 2 * mine;
         if (chunk >= n_chunks) break;
         ++turn;
-        const int target = targets[mine];
         const float factor = kRows == Rows::kUp ? factors[mine] : 1.f;
         const int buffer = group * 2 + (turn & 1);
         uint8_t* stage = chunks + buffer * kChunkBytes;
@@ -446,63 +603,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(
             stmatrix_x4_trans(at, pack_bf16(y[4 * i], y[4 * i + 1]), pack_bf16(y[4 * i + 2], y[4 * i + 3]),
                               pack_bf16(y[4 * i + 4], y[4 * i + 5]), pack_bf16(y[4 * i + 6], y[4 * i + 7]));
           }
-        } else if constexpr (kRows == Rows::kDown) {
-          // fp16 with an exponent per token and 32 channels: its largest finite value comes to lie in [2^14, 2^15).  Of the
-          // largest only the exponent is needed, two tokens' to a word.
-          uint32_t top[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float a[2];
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-              a[c] = fmaxf(fmaxf(fabsf(v[0][4 * i + c]), fabsf(v[0][4 * i + 2 + c])),
-                           fmaxf(fabsf(v[1][4 * i + c]), fabsf(v[1][4 * i + 2 + c])));
-            top[i] = (__float_as_uint(a[0]) >> 23) | (__float_as_uint(a[1]) >> 23 << 16);
-          }
-          bool infinite = false;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) infinite |= (top[i] & 0xffffu) == 255u || (top[i] >> 16) == 255u;
-          if (infinite) {  // by finite values alone
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              top[i] = 0;
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                uint32_t most = 0;
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                  const uint32_t e = __float_as_uint(v[m >> 1][4 * i + 2 * (m & 1) + c]) >> 23 & 255u;
-                  most = e < 255u && e > most ? e : most;
-                }
-                top[i] |= most << (16 * c);
-              }
-            }
-          }
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) top[i] = __vmaxu2(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            // 2^(141 - e) as long as that is a normal number (e >= 15).
-            const int e0 = max((int)(top[i] & 0xffffu), 15), e1 = max((int)(top[i] >> 16), 15);
-            const float s0 = __uint_as_float((uint32_t)(268 - e0) << 23), s1 = __uint_as_float((uint32_t)(268 - e1) << 23);
-            if (sub == 0) {
-              const int at = (buffer * kChunk + i * 8 + pick * 2) * 4 + quad;
-              chunk_exponents[at] = (int8_t)(141 - e0);
-              chunk_exponents[at + 4] = (int8_t)(141 - e1);
-            }
-            uint32_t out[4];
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              const int f = 4 * i + 2 * (m & 1);
-              out[m] = Mma16816<__half>::pack(v[m >> 1][f] * s0, v[m >> 1][f + 1] * s1);
-            }
-            const int row = i * 8 + line;
-            stmatrix_x4_trans(stage_addr + (uint32_t)(row * kRowBytes + (((quad * 4 + part) ^ (row & 7)) * 16)), out[0], out[1],
-                              out[2], out[3]);
-          }
         } else {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -531,28 +631,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(
         asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(threads_of_group) : "memory");
         // Whole runs of y's rows.  The other buffer takes the next chunk, so that one barrier a chunk is enough.
         uint4 data[kChunk / kRowsPerStep];
-        int to[kChunk / kRowsPerStep];  // row of y, -1: none
 #pragma unroll
         for (int i = 0; i < kChunk / kRowsPerStep; ++i) {
           const int row = i * kRowsPerStep + store_row;
           data[i] = *reinterpret_cast<const uint4*>(stage + row * kRowBytes + ((store_part ^ (row & 7)) * 16));
-          to[i] = __shfl_sync(0xffffffffu, target, row);
-          if (chunk * kChunk + row >= t.count || !ok || store_channel >= p.n) to[i] = -1;
         }
 #pragma unroll
         for (int i = 0; i < kChunk / kRowsPerStep; ++i) {
-          uint16_t* dst = reinterpret_cast<uint16_t*>(p.y) + to[i] * p.ldy + store_channel;
+          const int row = chunk * kChunk + i * kRowsPerStep + store_row;
+          if (row >= t.count || !ok || store_channel >= p.n) continue;
+          uint16_t* dst = reinterpret_cast<uint16_t*>(p.y) + (long long)(t.first + row) * p.ldy + store_channel;
           if (vec_store) {
-            if (to[i] >= 0) *reinterpret_cast<uint4*>(dst) = data[i];
-          } else if (to[i] >= 0) {
+            *reinterpret_cast<uint4*>(dst) = data[i];
+          } else {
             const uint32_t w[4] = {data[i].x, data[i].y, data[i].z, data[i].w};
 #pragma unroll
             for (int j = 0; j < 8; ++j)
               if (store_channel + j < p.n) dst[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
           }
-          if (kRows == Rows::kDown && store_part % 4 == 0 && to[i] >= 0)
-            q.exponents[(long long)to[i] * q.exponent_ld + store_channel / 32] =
-                chunk_exponents[(buffer * kChunk + i * kRowsPerStep + store_row) * 4 + store_part / 4];
         }
       }
       if (!released) {  // a group without a chunk of this tile
@@ -579,19 +675,27 @@ inline bool rows_fit_tma(const void* ptr, long long stride) {
   return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && stride % 8 == 0;
 }
 
-// Weight rows [experts][rows][k]; gated as runs of 8 gates and 8 ups, `rows` of each.
-inline int weight_map(CUtensorMap* out, const Product& p, int experts) {
-  const uint64_t row = (uint64_t)p.ldw * 2, expert = experts > 1 ? (uint64_t)p.w_expert * 2 : row;
-  if (p.gated) {
-    const uint64_t dims[5] = {(uint64_t)p.k, 8, 2, (uint64_t)p.n / 8, (uint64_t)experts};
-    const uint64_t strides[4] = {row, (uint64_t)p.n * row, 8 * row, expert};
-    const uint32_t box[5] = {64, 8, 2, 8, 1};
-    return cached_operand_map(out, 5, p.w, dims, strides, box);
+inline int weight_maps(WeightMaps* out, const Product& p, int experts, bool direct) {
+  const uint64_t row = (uint64_t)p.ldw * 2, expert = experts > 1 ? (uint64_t)p.w_expert * 2 : row, k = (uint64_t)p.k;
+  if (!p.gated && !direct) {
+    const uint64_t dims[3] = {k, (uint64_t)p.n, (uint64_t)experts};
+    const uint64_t strides[2] = {row, expert};
+    const uint32_t box[3] = {64, 128, 1};
+    return cached_operand_map(&out->all, 3, p.w, dims, strides, box);
   }
-  const uint64_t dims[3] = {(uint64_t)p.k, (uint64_t)p.n, (uint64_t)experts};
-  const uint64_t strides[2] = {row, expert};
-  const uint32_t box[3] = {64, 128, 1};
-  return cached_operand_map(out, 3, p.w, dims, strides, box);
+  // Runs: [8 rows][gate, up] or [8 rows 4 apart][4 rows].
+  const uint32_t inner = p.gated ? 2 : 4, runs = p.gated ? 8 : 4;
+  const int run = p.gated ? 8 : 32, whole = p.n / run, rest = p.n - whole * run;
+  const uint64_t strides[4] = {p.gated ? row : 4 * row, p.gated ? (uint64_t)p.n * row : row, (uint64_t)run * row, expert};
+  const uint32_t box[5] = {64, 8, inner, runs, 1}, one[5] = {64, 8, inner, 1, 1};
+  const uint64_t dims[5] = {k, 8, inner, (uint64_t)(whole > 0 ? whole : 1), (uint64_t)experts};
+  // A weight of less than a run has no whole one; what stands in its place is never loaded.
+  const uint64_t rest_rows = (uint64_t)(p.gated ? rest : rest / 4);
+  const uint64_t rest_dims[5] = {k, rest > 0 ? rest_rows : 8, inner, 1, (uint64_t)experts};
+  const __nv_bfloat16* rest_base = rest > 0 ? p.w + (long long)whole * run * p.ldw : p.w;
+  if (int rc = cached_operand_map(&out->all, 5, p.w, dims, strides, box)) return rc;
+  if (int rc = cached_operand_map(&out->run, 5, p.w, dims, strides, one)) return rc;
+  return cached_operand_map(&out->rest, 5, rest_base, rest_dims, strides, one);
 }
 inline int row_map(CUtensorMap* out, const Product& p, long long rows, int box_rows) {
   const uint64_t dims[2] = {(uint64_t)p.k, (uint64_t)rows};
@@ -601,23 +705,28 @@ inline int row_map(CUtensorMap* out, const Product& p, long long rows, int box_r
 }
 // What the pair kernel's loads ask of the operands.
 inline bool wide_takes(const Product& p) {
-  return p.k % 8 == 0 && rows_fit_tma(p.x, p.ldx) && rows_fit_tma(p.w, p.ldw) && p.w_expert % 8 == 0 &&
-         (!p.gated || p.n % 8 == 0);
+  return p.k % 8 == 0 && rows_fit_tma(p.x, p.ldx) && rows_fit_tma(p.w, p.ldw) && p.w_expert % 8 == 0;
 }
 
-template <Rows kRows, bool kGated>
-int launch_wide(const CUtensorMap& map_w, const CUtensorMap& map_x, const WideParams& q, long long most_tiles,
+// Whether finished values may go to y (and come from the residual) by runs of four.
+inline bool direct_takes(const Product& p) {
+  return !p.gated && p.n % 4 == 0 && p.ldy % 4 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 7) == 0 &&
+         (p.residual == nullptr || (p.ldr % 4 == 0 && (reinterpret_cast<uintptr_t>(p.residual) & 7) == 0));
+}
+
+template <Rows kRows, bool kGated, bool kDirect>
+int launch_wide(const WeightMaps& maps, const CUtensorMap& map_x, const WideParams& q, long long most_tiles,
                 cudaStream_t stream) {
   static bool configured[64] = {false};
   int dev = 0;
   MIE_CUDA(cudaGetDevice(&dev));
   if (dev >= 0 && dev < 64 && !configured[dev]) {
-    MIE_CUDA(cudaFuncSetAttribute(product_wide_kernel<kRows, kGated>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem));
+    MIE_CUDA(cudaFuncSetAttribute(product_wide_kernel<kRows, kGated, kDirect>, cudaFuncAttributeMaxDynamicSharedMemorySize, wide_smem<kDirect>()));
     configured[dev] = true;
   }
   const long long most = sm_count() / 2;
-  MIE_CUDA(launch_chained(product_wide_kernel<kRows, kGated>, dim3((unsigned)(2 * (most_tiles < most ? most_tiles : most))),
-                          dim3(wide_threads<kRows>()), kWideSmem, stream, map_w, map_x, q));
+  MIE_CUDA(launch_chained(product_wide_kernel<kRows, kGated, kDirect>, dim3((unsigned)(2 * (most_tiles < most ? most_tiles : most))),
+                          dim3(wide_threads<kRows>()), wide_smem<kDirect>(), stream, maps, map_x, q));
   MIE_LAUNCH_CHECK("product_wide_kernel");
   return MIE_OK;
 }

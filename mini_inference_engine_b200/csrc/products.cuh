@@ -28,10 +28,10 @@ struct Product {
   int m, n, k;  // rows, columns of y, length of the sums; a gated weight has 2 n rows
   int activation, gated, wide;
   // Over experts: the tiles, how many there are, and for a sorted row the row of x that it reads (source, divided by
-  // source_divisor), the row of y that it writes (target) and its factor (by source).
+  // source_divisor; its own without one) and its factor (by source).
   const RowTile* tiles;
   const int* tile_count;
-  const int *source, *target;
+  const int* source;
   int source_divisor;
   const float* factor;
   int* status;
@@ -148,12 +148,11 @@ __global__ void __launch_bounds__(128) product_any_kernel(const Product p) {
         if (p.gated) v *= u;
         const long long sorted = rows.first + r;
         if (kRouted && p.factor != nullptr) v *= p.factor[p.source[sorted]];
-        const long long target = kRouted && p.target != nullptr ? p.target[sorted] : sorted;
-        if (p.residual != nullptr) v += __bfloat162float(p.residual[target * p.ldr + col]);
+        if (p.residual != nullptr) v += __bfloat162float(p.residual[sorted * p.ldr + col]);
         if (p.wide)
-          reinterpret_cast<float*>(p.y)[target * p.ldy + col] = v;
+          reinterpret_cast<float*>(p.y)[sorted * p.ldy + col] = v;
         else
-          reinterpret_cast<__nv_bfloat16*>(p.y)[target * p.ldy + col] = __float2bfloat16_rn(v);
+          reinterpret_cast<__nv_bfloat16*>(p.y)[sorted * p.ldy + col] = __float2bfloat16_rn(v);
       }
     }
   }
