@@ -9,6 +9,7 @@
 //
 // A pair's order among its expert's rows is whatever the counters gave; every row of a product is computed by itself, so
 // the results do not depend on it.  Ids outside [0, experts) take no part: -1 says "no expert", others also set a status bit.
+#include "product_narrow.cuh"
 #include "product_wide.cuh"
 #include "products.cuh"
 #include "rows.cuh"
@@ -226,13 +227,16 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const CombineParams
 // Where the parts of the scratch begin.
 struct Scratch {
   long long order, position, tiles, tile_count, hidden, exponents, rows, total;
-  Scratch(long long pairs, int experts, int width, int ff) {
+  Scratch(long long tokens, int top_k, int experts, int width, int ff) {
+    const long long pairs = tokens * top_k;
     total = 0;
     order = take(pairs * 4);
     position = take(pairs * 4);
     tiles = take(most_tiles(pairs, experts, kAnyTile) * (long long)sizeof(RowTile));
     tile_count = take(4);
-    hidden = take(pairs * ff * 2);
+    // Few rows: a hidden row of every token for every expert in use.
+    const long long few = tokens > kFewRoutedRows ? 0 : (pairs < experts ? pairs : experts) * (tokens > 16 ? 32 : 16);
+    hidden = take((pairs > few ? pairs : few) * ff * 2);
     exponents = take(pairs * exponent_ld(width));
     rows = take(pairs * width * 4);
   }
@@ -266,6 +270,31 @@ int launch_plan(const PlanParams& plan, cudaStream_t stream) {
   return MIE_OK;
 }
 
+// Few rows: every expert in use for all of them (see product_narrow.cuh).
+template <int BN>
+int launch_routed_few(const Product& up, const Product& out, FewParams q, cudaStream_t stream) {
+  const int rows = up.m;
+  CUtensorMap map_w, map_x;
+  q.p = up;
+  q.weight_tiles = (up.n + 63) / 64;
+  const long long pairs = (long long)rows * q.top_k, most = pairs < q.experts ? pairs : q.experts;
+  if (int rc = few_weight_map(&map_w, up, q.experts)) return rc;
+  if (int rc = row_map(&map_x, up, rows, BN)) return rc;
+  const int ctas = FewSmem<BN, Few::kUp>::kCtasPerSm;
+  if (int rc = launch_few<BN, Few::kUp, true>(map_w, map_x, q, most * q.weight_tiles,
+                                              few_split(most * q.weight_tiles, (up.k + 63) / 64, ctas), stream))
+    return rc;
+  q.p = out;
+  q.weight_tiles = (out.n + 127) / 128;
+  if (int rc = few_weight_map(&map_w, out, q.experts)) return rc;
+  const uint64_t dims[3] = {(uint64_t)out.k, (uint64_t)BN, (uint64_t)most};
+  const uint64_t strides[2] = {(uint64_t)out.ldx * 2, (uint64_t)out.ldx * 2 * BN};
+  const uint32_t box[3] = {64, (uint32_t)BN, 1};
+  if (int rc = cached_operand_map(&map_x, 3, out.x, dims, strides, box)) return rc;
+  return launch_few<BN, Few::kDown, false>(map_w, map_x, q, q.weight_tiles,
+                                           few_split(q.weight_tiles, (int)most * ((out.k + 63) / 64), ctas), stream);
+}
+
 int launch_any(const Product& p, long long tiles, cudaStream_t stream) {
   MIE_CUDA(launch_chained(product_any_kernel<true>,
                           dim3((unsigned)((p.n + kAnyTile - 1) / kAnyTile), (unsigned)(tiles < 65535 ? tiles : 65535)),
@@ -281,7 +310,7 @@ using namespace mie;
 
 extern "C" int64_t mie_expert_scratch_bytes(int32_t tokens, int32_t top_k, int32_t experts, int32_t width, int32_t ff) {
   if (tokens < 0 || top_k < 1 || experts < 1 || width < 1 || ff < 1) return 0;
-  return Scratch((long long)tokens * top_k, experts, width, ff).total;
+  return Scratch(tokens, top_k, experts, width, ff).total;
 }
 
 extern "C" int mie_expert_mlp(const void* x, int64_t ldx, mie_index_t ids, const float* weights, const void* gate_up,
@@ -299,7 +328,7 @@ extern "C" int mie_expert_mlp(const void* x, int64_t ldx, mie_index_t ids, const
                 "a row is longer than its stride");
   MIE_CHECK_ARG(activation >= MIE_ACT_NONE && activation <= MIE_ACT_RELU, "unknown activation %d", activation);
   const int pairs = tokens * top_k;
-  const Scratch s(pairs, experts, width, ff);
+  const Scratch s(tokens, top_k, experts, width, ff);
   MIE_CHECK_ARG(scratch_bytes >= s.total, "scratch of %lld bytes, %lld needed", (long long)scratch_bytes, s.total);
   MIE_CHECK_ARG((reinterpret_cast<uintptr_t>(scratch) & 255) == 0, "scratch must be 256-byte aligned");
   if (tokens == 0) return MIE_OK;
@@ -327,6 +356,13 @@ extern "C" int mie_expert_mlp(const void* x, int64_t ldx, mie_index_t ids, const
                         (const __nv_bfloat16*)residual, ldr, (__nv_bfloat16*)y, ldy, tokens, top_k, width};
 
   const bool wide = wide_takes(up) && wide_takes(out) && direct_takes(out);
+  if (wide && tokens <= kFewRoutedRows) {
+    FewParams few = {};
+    few.ids = IndexView(ids), few.weights = weights, few.top_k = top_k, few.experts = experts;
+    up.m = out.m = tokens;
+    out.y = y, out.ldy = ldy, out.residual = (const __nv_bfloat16*)residual, out.ldr = ldr;
+    return tokens <= 16 ? launch_routed_few<16>(up, out, few, stream) : launch_routed_few<32>(up, out, few, stream);
+  }
   const int tile_rows = wide ? kWideRows : kAnyTile;
   const long long tiles = s.most_tiles(pairs, experts, tile_rows);
   const PlanParams plan{IndexView(ids), pairs, top_k, experts, tile_rows, order, (int*)(base + s.position), (RowTile*)(base + s.tiles),

@@ -1,9 +1,12 @@
 // Projections with bias, activation or gate, and residual in their epilogue.
+#include "product_narrow.cuh"
 #include "product_wide.cuh"
 #include "products.cuh"
 
 namespace mie {
 namespace {
+
+constexpr int kFewRows = 128;
 
 int launch_any(const Product& p, cudaStream_t stream) {
   const int row_tiles = (p.m + kAnyTile - 1) / kAnyTile;
@@ -44,6 +47,26 @@ int launch_dense_wide(const Product& p, cudaStream_t stream) {
                   : launch_wide<Rows::kDense, false, false>(maps, map_x, q, tiles, stream);
 }
 
+template <int BN, bool kGated>
+int launch_dense_few(const Product& p, cudaStream_t stream) {
+  FewParams q = {};
+  q.p = p;
+  const long long tiles = (p.n + (kGated ? 63 : 127)) / (kGated ? 64 : 128);
+  CUtensorMap map_w, map_x;
+  if (int rc = few_weight_map(&map_w, p, 1)) return rc;
+  if (int rc = row_map(&map_x, p, p.m, BN)) return rc;
+  return launch_few<BN, Few::kDense, kGated>(map_w, map_x, q, tiles,
+                                             few_split(tiles, (p.k + 63) / 64, FewSmem<BN, Few::kDense>::kCtasPerSm), stream);
+}
+
+template <bool kGated>
+int launch_dense_few(const Product& p, cudaStream_t stream) {
+  if (p.m <= 16) return launch_dense_few<16, kGated>(p, stream);
+  if (p.m <= 32) return launch_dense_few<32, kGated>(p, stream);
+  if (p.m <= 64) return launch_dense_few<64, kGated>(p, stream);
+  return launch_dense_few<128, kGated>(p, stream);
+}
+
 }  // namespace
 }  // namespace mie
 
@@ -66,5 +89,7 @@ extern "C" int mie_fused_linear(const void* x, int64_t ldx, const void* w, int64
   p.y = y, p.ldy = ldy;
   p.m = m, p.n = n, p.k = k;
   p.activation = activation, p.gated = gated != 0, p.status = status;
-  return wide_takes(p) ? launch_dense_wide(p, stream) : launch_any(p, stream);
+  if (!wide_takes(p)) return launch_any(p, stream);
+  if (m <= kFewRows) return p.gated ? launch_dense_few<true>(p, stream) : launch_dense_few<false>(p, stream);
+  return launch_dense_wide(p, stream);
 }

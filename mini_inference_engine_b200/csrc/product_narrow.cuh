@@ -1,0 +1,419 @@
+// Products of few rows: the weights are streamed once, 128 rows of them a CTA as the M of a tcgen05 accumulator whose N are the
+// BN rows of x.  Bound by HBM, and by the time from the kernel before to the first weights and from the last weights to the
+// end.  K is cut across a cluster of up to 8 CTAs where the weight has too few tiles to fill the GPU; the parts' sums meet in
+// shared memory, in rank order.
+//
+//   kDense  y = act(x W^T + b) + res, gated or not
+//   kUp     routed: every expert that any row is sent to, for all rows: hidden[u][row] = act(G x) * (U x), u the expert's
+//           place among those in use.  Rows of x that are not sent there are computed too (the weights are what counts), not
+//           used.
+//   kDown   routed: y[row] = res + sum_u w[row, u] D_u hidden[u][row].  The sum over the experts is one long K, cut across the
+//           cluster; where an expert ends its part is taken out of tensor memory and added, with its weights, to the rows
+//           that are sent there and to no others (an expert's infinities stay with its rows).
+//
+// Which experts are in use every CTA finds out by itself from the ids, a few hundred at most.  kUp lets the kernel after it
+// start behind its own wait for the kernels before: kDown may read the ids, and ask for its first weights, while kUp runs.
+#pragma once
+
+#include "products.cuh"
+#include "umma.cuh"
+
+namespace mie {
+namespace {
+
+enum class Few { kDense, kUp, kDown };
+
+constexpr int kFewThreads = 192;     // 4 finishing warps, TMA producer, MMA issuer
+constexpr int kFewRoutedRows = 32;   // most rows of the routed form
+constexpr int kFewPairs = kFewRoutedRows * MIE_MAX_TOP_K;
+
+template <int BN, Few kKind>
+struct FewSmem {
+  static constexpr int kStageBytes = 128 * 128 + BN * 128;
+  static constexpr int kCtasPerSm = BN <= 64 ? 2 : 1;
+  static constexpr int kRouting = kKind == Few::kDense ? 0 : kFewPairs * 6 + MIE_MAX_EXPERTS * 2 + 256;
+  static constexpr int kStages = ((kCtasPerSm == 2 ? 110 : 220) * 1024 - kRouting) / kStageBytes;
+  static constexpr int kAcc = kKind == Few::kDown ? 4 : 1;  // accumulators in tensor memory
+  static constexpr int kAccColumns = BN < 32 ? 32 : BN;
+  static constexpr int kTotal = kStages * kStageBytes + kRouting + (2 * kStages + 2 * kAcc) * 8 + 16 + 1024;
+  static_assert(kTotal <= (kCtasPerSm == 2 ? 113 : 227) * 1024, "shared memory of an SM");
+  static_assert(kStages * kStageBytes >= BN * 128 * 4, "the ring also parks the fp32 sums");
+};
+
+struct FewParams {
+  Product p;
+  // Routed.
+  IndexView ids;  // [rows, top_k]
+  const float* weights;
+  int top_k, experts, weight_tiles;
+};
+
+// The experts in use, ascending, and the pairs' experts and weights, in shared memory.
+struct Routing {
+  int16_t* used;      // [MIE_MAX_EXPERTS]
+  int16_t* expert;    // [rows * top_k], -1: none
+  float* weight;      // [rows * top_k]
+  uint32_t* bitmap;   // [32]
+  int* count;
+};
+__device__ __forceinline__ Routing routing_at(uint8_t* base) {
+  Routing r;
+  r.weight = reinterpret_cast<float*>(base);
+  r.used = reinterpret_cast<int16_t*>(base + kFewPairs * 4);
+  r.expert = r.used + MIE_MAX_EXPERTS;
+  r.bitmap = reinterpret_cast<uint32_t*>(r.expert + kFewPairs);
+  r.count = reinterpret_cast<int*>(r.bitmap + 32);
+  return r;
+}
+__device__ __forceinline__ int find_routing(const Routing& r, const FewParams& q, bool report) {
+  const int pairs = q.p.m * q.top_k, tid = threadIdx.x;
+  if (tid < 32) r.bitmap[tid] = 0;
+  __syncthreads();
+  for (int i = tid; i < pairs; i += kFewThreads) {
+    const int row = i / q.top_k;
+    const long long e = q.ids.at(row, i - row * q.top_k);
+    const bool valid = e >= 0 && e < q.experts;
+    if (!valid && e != -1 && report) raise_status(q.p.status, MIE_STATUS_BAD_EXPERT);
+    r.expert[i] = valid ? (int16_t)e : (int16_t)-1;
+    r.weight[i] = q.weights[i];
+    if (valid) atomicOr(&r.bitmap[e >> 5], 1u << (e & 31));
+  }
+  __syncthreads();
+  if (tid < 32) {
+    uint32_t word = r.bitmap[tid];
+    int before = __popc(word);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, before, o);
+      if (tid >= o) before += other;
+    }
+    if (tid == 31) *r.count = before;
+    before -= __popc(word);
+    for (; word != 0; word &= word - 1) r.used[before++] = (int16_t)(tid * 32 + __ffs(word) - 1);
+  }
+  __syncthreads();
+  return *r.count;
+}
+
+template <int kSplit>
+__device__ __forceinline__ float4 sum_parts(uint32_t park, int at) {
+  float4 part[kSplit];
+#pragma unroll
+  for (int peer = 0; peer < kSplit; ++peer) part[peer] = ld_cluster_f4(park + (uint32_t)at * 4u, (uint32_t)peer);
+  float4 sum = part[0];
+#pragma unroll
+  for (int peer = 1; peer < kSplit; ++peer) {
+    sum.x += part[peer].x;
+    sum.y += part[peer].y;
+    sum.z += part[peer].z;
+    sum.w += part[peer].w;
+  }
+  return sum;
+}
+__device__ __forceinline__ float4 sum_parts(uint32_t park, int at, int split) {
+  return split == 8 ? sum_parts<8>(park, at) : split == 4 ? sum_parts<4>(park, at)
+         : split == 2 ? sum_parts<2>(park, at) : sum_parts<1>(park, at);
+}
+
+// grid = (tiles, split), cluster = (1, split).
+template <int BN, Few kKind, bool kGated>
+__global__ void __launch_bounds__(kFewThreads, FewSmem<BN, kKind>::kCtasPerSm)
+    product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const FewParams q) {
+  using S = FewSmem<BN, kKind>;
+  constexpr int kStages = S::kStages, kAcc = S::kAcc;
+  constexpr int kTmemColumns = kAcc * S::kAccColumns;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(ring + kStages * S::kStageBytes);
+  uint64_t* empty_bar = full_bar + kStages;
+  uint64_t* acc_full = empty_bar + kStages;
+  uint64_t* acc_empty = acc_full + kAcc;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + kAcc);
+  const Routing routing = routing_at(reinterpret_cast<uint8_t*>(tmem_slot + 4));
+  const Product& p = q.p;
+  const int warp = uniform_warp_index(), lane = threadIdx.x & 31;
+  const int split = gridDim.y, rank = blockIdx.y;
+  const int blocks = (p.k + 63) / 64;  // of an expert's K
+
+  if (warp == 4 && lane == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < kAcc; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], 4);
+    }
+    mbar_fence_init();
+    tma_prefetch_desc(&map_w);
+    tma_prefetch_desc(&map_x);
+  }
+  if (warp == 5) {
+    tmem_alloc(tmem_slot, kTmemColumns);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // kDown reads the ids and weights ahead of its wait: kUp, whose hidden rows it waits for, has waited for what wrote them.
+  if (kKind != Few::kUp) chain_release();
+  if (kKind != Few::kDown) chain_wait();
+  if (kKind == Few::kUp) chain_release();
+  const int used = kKind == Few::kDense ? 1 : find_routing(routing, q, kKind == Few::kUp);
+
+  const int tile = kKind == Few::kUp ? (int)blockIdx.x % q.weight_tiles : (int)blockIdx.x;
+  const int place = kKind == Few::kUp ? (int)blockIdx.x / q.weight_tiles : 0;
+  const bool idle = kKind == Few::kUp && place >= used;  // the same for a whole cluster
+  const int total = kKind == Few::kDown ? used * blocks : blocks;
+  const int first = idle ? 0 : (int)((long long)total * rank / split);
+  const int count = idle ? 0 : (int)((long long)total * (rank + 1) / split) - first;
+  const int expert = kKind == Few::kUp && !idle ? routing.used[place] : 0;
+
+  bool ok = true;
+  const uint32_t park = smem_u32(ring);
+  if (warp == 4) {
+    if (lane == 0) {
+      const uint64_t policy = l2_evict_first_policy();  // weights are streamed once per call
+      int requested = 0;
+      auto request_weights = [&](int i) {
+        const int s = i % kStages, at = first + i;
+        const int unit = kKind == Few::kDown ? at / blocks : 0, b = kKind == Few::kDown ? at - unit * blocks : at;
+        const int e = kKind == Few::kDown ? routing.used[unit] : expert;
+        uint8_t* dst = ring + (size_t)s * S::kStageBytes;
+        mbar_expect_tx(&full_bar[s], S::kStageBytes);
+        if (kGated) {
+          tma_load_3d_hint(dst, &map_w, &full_bar[s], b * 64, tile * 64, e, policy);
+          tma_load_3d_hint(dst + 8192, &map_w, &full_bar[s], b * 64, p.n + tile * 64, e, policy);
+        } else {
+          tma_load_3d_hint(dst, &map_w, &full_bar[s], b * 64, tile * 128, e, policy);
+        }
+      };
+      if (kKind == Few::kDown) {
+        for (; requested < count && requested < kStages; ++requested) request_weights(requested);
+        chain_wait();
+      }
+      for (int i = 0; i < count; ++i) {
+        const int s = i % kStages, at = first + i;
+        if (i >= requested) {
+          if (!mbar_wait_bounded(&empty_bar[s], ((i / kStages) & 1u) ^ 1u)) {
+            raise_status(p.status, MIE_STATUS_WAIT_TIMEOUT);
+            break;
+          }
+          request_weights(i);
+        }
+        uint8_t* dst = ring + (size_t)s * S::kStageBytes + 128 * 128;
+        if (kKind == Few::kDown) {
+          const int unit = at / blocks;
+          tma_load_3d(dst, &map_x, &full_bar[s], (at - unit * blocks) * 64, 0, unit);
+        } else {
+          tma_load_2d(dst, &map_x, &full_bar[s], at * 64, 0);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 5) {
+    constexpr uint32_t idesc = instr_desc_bf16(128, BN, 0, 0);
+    int part = 0;  // runs of one expert
+    for (int i = 0; i < count; ++i) {
+      const int s = i % kStages;
+      const int in_unit = kKind == Few::kDown ? (first + i) % blocks : i;
+      const bool opens = i == 0 || in_unit == 0;
+      const bool closes = i == count - 1 || in_unit == blocks - 1;
+      const int acc = part % kAcc;
+      if (opens && part >= kAcc && !warp_wait_bounded(&acc_empty[acc], ((part / kAcc) & 1u) ^ 1u)) {
+        raise_status(p.status, MIE_STATUS_WAIT_TIMEOUT);
+        break;
+      }
+      if (!warp_wait_bounded(&full_bar[s], (i / kStages) & 1u)) {
+        raise_status(p.status, MIE_STATUS_WAIT_TIMEOUT);
+        break;
+      }
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t a = smem_u32(ring + (size_t)s * S::kStageBytes);
+        const uint64_t da = smem_desc_k128(a), db = smem_desc_k128(a + 128 * 128);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          umma_f16(tmem + acc * S::kAccColumns, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc,
+                   opens && k == 0 ? 0u : 1u);
+        umma_commit(&empty_bar[s]);
+        if (closes) umma_commit(&acc_full[acc]);
+      }
+      __syncwarp();
+      if (closes) ++part;
+    }
+  } else {
+    // One weight row a thread.
+    const int row = warp * 32 + lane;
+    const uint32_t lane_addr = tmem + ((uint32_t)(warp * 32) << 16);
+    float sum[BN];
+#pragma unroll
+    for (int j = 0; j < BN; ++j) sum[j] = 0.f;
+    if constexpr (kKind == Few::kDown) {
+      int part = 0;
+      for (int at = first; at < first + count; ++part) {
+        const int unit = at / blocks, acc = part % kAcc;
+        at = (unit + 1) * blocks;
+        // Lane j: the weight of row j for this expert, and whether it is sent there.
+        float factor = 0.f;
+        bool sent = false;
+        if (lane < p.m) {
+          const int e = routing.used[unit];
+          for (int j = 0; j < q.top_k; ++j) {
+            if (routing.expert[lane * q.top_k + j] == e) {
+              factor += routing.weight[lane * q.top_k + j];
+              sent = true;
+            }
+          }
+        }
+        const uint32_t rows = __ballot_sync(0xffffffffu, sent);
+        if (ok && !warp_wait_bounded(&acc_full[acc], (part / kAcc) & 1u)) {
+          ok = false;
+          raise_status(p.status, MIE_STATUS_WAIT_TIMEOUT);
+        }
+        tc_fence_after();
+        float v[BN];
+        if constexpr (BN == 32)
+          tmem_ld32(lane_addr + acc * S::kAccColumns, v);
+        else
+          tmem_ld16(lane_addr + acc * S::kAccColumns, v);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[acc]);
+#pragma unroll
+        for (int j = 0; j < BN; ++j) {
+          const float f = __shfl_sync(0xffffffffu, factor, j);
+          if ((rows >> j) & 1u) sum[j] = fmaf(f, v[j], sum[j]);
+        }
+      }
+    } else if (count > 0) {
+      ok = warp_wait_bounded(&acc_full[0], 0);
+      if (!ok) raise_status(p.status, MIE_STATUS_WAIT_TIMEOUT);
+      tc_fence_after();
+      if constexpr (BN >= 32) {
+#pragma unroll
+        for (int c = 0; c < BN; c += 32) tmem_ld32(lane_addr + c, *reinterpret_cast<float(*)[32]>(&sum[c]));
+      } else {
+        tmem_ld16(lane_addr, *reinterpret_cast<float(*)[16]>(&sum[0]));
+      }
+      tmem_ld_wait();
+    }
+    // The ring is idle: the last MMA has been waited for by every finishing warp (one that gave up stores nothing).
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < BN; ++j)
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(park + (uint32_t)((j * 128 + row) * 4)), "f"(sum[j]) : "memory");
+  }
+  __syncwarp();
+  if (kKind == Few::kDown) chain_wait();  // every thread: the residual and y belong to the kernels before as well
+  cluster_sync_all();
+  if (warp < 4 && !idle) {
+    // Units of four channels of a row, over all CTAs of the cluster.
+    constexpr int kFours = kGated ? 16 : 32;
+    const int channel0 = tile * (kGated ? 64 : 128);
+    for (int i = rank * 128 + (int)threadIdx.x; i < p.m * kFours; i += split * 128) {
+      const int row = i / kFours, four = i % kFours, channel = channel0 + four * 4;
+      const float4 s = sum_parts(park, row * 128 + four * 4, split);
+      float v[4] = {s.x, s.y, s.z, s.w};
+      float u[4] = {1.f, 1.f, 1.f, 1.f};
+      if (kGated) {
+        const float4 up = sum_parts(park, row * 128 + 64 + four * 4, split);
+        u[0] = up.x, u[1] = up.y, u[2] = up.z, u[3] = up.w;
+      }
+      if (channel >= p.n || !ok) continue;
+      const int valid = p.n - channel < 4 ? p.n - channel : 4;
+      if (kKind == Few::kDense && p.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (j >= valid) break;
+          v[j] += __bfloat162float(p.bias[channel + j]);
+          if (kGated) u[j] += __bfloat162float(p.bias[p.n + channel + j]);
+        }
+      }
+      if (kKind != Few::kDown) activate_all(p.activation, v);
+      if (kGated) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] *= u[j];
+      }
+      const long long to = kKind == Few::kUp ? (long long)place * BN + row : row;
+      if (kKind != Few::kUp && p.residual != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j < valid) v[j] += __bfloat162float(p.residual[to * p.ldr + channel + j]);
+      }
+      __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(p.y) + to * p.ldy + channel;
+      if (valid == 4 && (reinterpret_cast<uintptr_t>(y) & 7) == 0) {
+        *reinterpret_cast<uint2*>(y) = make_uint2(Mma16816<__nv_bfloat16>::pack(v[0], v[1]), Mma16816<__nv_bfloat16>::pack(v[2], v[3]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j < valid) y[j] = __float2bfloat16_rn(v[j]);
+      }
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();  // no CTA leaves while another may still read its sums
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemColumns);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+// Weight rows [experts][n or 2 n][k]; any row count.
+inline int few_weight_map(CUtensorMap* out, const Product& p, int experts) {
+  const uint64_t row = (uint64_t)p.ldw * 2;
+  const uint64_t dims[3] = {(uint64_t)p.k, (uint64_t)p.n * (p.gated ? 2 : 1), (uint64_t)experts};
+  const uint64_t strides[2] = {row, experts > 1 ? (uint64_t)p.w_expert * 2 : row};
+  const uint32_t box[3] = {64, p.gated ? 64u : 128u, 1};
+  return cached_operand_map(out, 3, p.w, dims, strides, box);
+}
+
+template <int BN, Few kKind, bool kGated>
+int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x, const FewParams& q, long long tiles, int split,
+               cudaStream_t stream) {
+  using S = FewSmem<BN, kKind>;
+  static bool configured[64] = {false};
+  int dev = 0;
+  MIE_CUDA(cudaGetDevice(&dev));
+  if (dev >= 0 && dev < 64 && !configured[dev]) {
+    MIE_CUDA(cudaFuncSetAttribute(product_few_kernel<BN, kKind, kGated>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  S::kTotal));
+    configured[dev] = true;
+  }
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)tiles, (unsigned)split, 1);
+  config.blockDim = dim3(kFewThreads, 1, 1);
+  config.dynamicSmemBytes = S::kTotal;
+  config.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = (unsigned)split;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = chained_launch_enabled() ? 2 : 1;
+  prefer_shared_carveout(reinterpret_cast<const void*>(product_few_kernel<BN, kKind, kGated>));
+  MIE_CUDA(cudaLaunchKernelEx(&config, product_few_kernel<BN, kKind, kGated>, map_w, map_x, q));
+  MIE_LAUNCH_CHECK("product_few_kernel");
+  return MIE_OK;
+}
+
+// CTAs a tile's K is cut over: as many, in powers of two, as surely run at once and have a few blocks each.
+inline int few_split(long long tiles, int blocks, int ctas_per_sm) {
+  const long long slots = (long long)ctas_per_sm * sm_count() * 9 / 10;
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= slots && blocks >= 4 * split) split *= 2;
+  return split;
+}
+
+}  // namespace
+}  // namespace mie
