@@ -293,17 +293,26 @@ def view4_arg(tensor: torch.Tensor | None) -> View4T:
     return View4T(tensor.data_ptr(), (c_int64 * 4)(*tensor.stride()))
 
 
+# The handle of the current stream without a Stream object around it: 0.1 us instead of 2.4 us a call.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_arg(device: torch.device | None = None) -> c_void_p:
-    return c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    if _raw_stream is None or device is None or device.index is None:
+        return c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    return c_void_p(_raw_stream(device.index))
 
 
 _HERE = contextlib.nullcontext()
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def on_device(device: torch.device):
     """Context in which launches go to ``device``, which need not be the current one."""
 
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == _current_device() else torch.cuda.device(device)
 
 
 def ptr(tensor: torch.Tensor | None) -> c_void_p:

@@ -4,21 +4,26 @@
 //   groups: the top_groups groups whose group_best largest c add up to most stay in the choice
 //   ids = the top_k experts by c, descending, equal ones by their index;   w = s[ids] (/ their sum) * scale
 //
-// A warp takes a token and keeps its logits in registers; a choice is one maximum over the warp (`redux.sync`) and one
-// minimum over the indices that have it, so that equal values go to the lowest index.
+// 8, 16 or 32 lanes take a token (32 / lanes of them a warp), runs of V experts a lane, so that the lowest lane that has the
+// largest value has the lowest index.  Every lane sorts its run once; a choice is then one maximum over the token's lanes'
+// heads, and the lane that has it moves on.  Little data and many dependent steps: bound by instruction issue for many tokens
+// and by latency for few.
 //
 // The choice is that of 64 bits.  Without a bias, and with groups judged by their best expert, the order of the scores is the
-// order of the logits, which are compared as they are.  Otherwise c is computed in 32 bits with an error below 2^-20 (1 + |c|)
-// (exponential 2 ulp, its argument's rounding, a sum of up to 1024 terms, a quotient, the bias' addition; each at most a few
-// 2^-24 of a value in [0, 1] or of c).  Where two values that decide something are nearer than twice that and do not come
-// from equal logits and biases, the warp decides the token again in 64 bits.
+// order of the logits, which are compared as they are.  Otherwise c is computed in 32 bits with an error below 2^-19 (1 + |c|)
+// (approximate exponential and reciprocal 2^-22 each, the argument's rounding, a sum of up to 1024 terms, the bias' addition,
+// of a value in [0, 1] or of c).  Where two values that decide something are nearer than twice that and do not come from
+// equal logits and biases, the choice goes on to whatever is as near, and those candidates are ordered by c in 64 bits (all
+// experts, where there are more than 32).  Groups that are as near are decided again first.
 #include "common.cuh"
+#include "glue.cuh"
 
 namespace mie {
 namespace {
 
-constexpr int kRouteWarps = 8;
-constexpr float kUncertain = 1.9073486e-6f;  // 2^-19
+constexpr int kRouteWarps = 4;
+constexpr float kUncertain = 3.8146973e-6f;  // 2^-18
+constexpr uint32_t kAll = 0xffffffffu;
 
 struct RouteParams {
   const void* logits;
@@ -32,73 +37,122 @@ struct RouteParams {
 
 // Monotonic integers of floating values: above 1 for every number; NaN is 1, below -inf and above 0, "not to be chosen".
 __device__ __forceinline__ uint32_t order_key(float v) {
-  const uint32_t u = __float_as_uint(v == 0.f ? 0.f : v);  // -0 equals 0
-  return v != v ? 1u : (u >> 31) ? ~u : u | 0x80000000u;
+  const uint32_t u = __float_as_uint(v + 0.f);  // -0 equals 0
+  return v != v ? 1u : u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
-  return k == 1u ? __uint_as_float(0x7fc00000u) : __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
+  return k <= 1u ? __uint_as_float(0x7fc00000u) : __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
 }
 __device__ __forceinline__ unsigned long long order_key(double v) {
-  const unsigned long long u = (unsigned long long)__double_as_longlong(v == 0.0 ? 0.0 : v);
+  const unsigned long long u = (unsigned long long)__double_as_longlong(v + 0.0);
   return v != v ? 1ull : (u >> 63) ? ~u : u | 0x8000000000000000ull;
-}
-__device__ __forceinline__ uint32_t warp_top(uint32_t key) { return __reduce_max_sync(0xffffffffu, key); }
-__device__ __forceinline__ unsigned long long warp_top(unsigned long long key) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
-    key = other > key ? other : key;
-  }
-  return key;
 }
 __device__ __forceinline__ bool far_apart(float a, float b, float size) { return fabsf(a - b) > kUncertain * (1.f + size); }
 
-// A row's choice in 64 bits (see above), by the whole warp; `scratch` and `chosen` are shared memory of the warp.
-template <typename T>
-__device__ __noinline__ void choose_again(const RouteParams& p, const T* row, float top, double* scratch, int* chosen) {
-  const int lane = threadIdx.x & 31, size = p.experts / p.groups;
-  double sum = 0.0;
-  if (!p.sigmoid) {
-    for (int e = lane; e < p.experts; e += 32) sum += exp((double)to_float<T>(row[e]) - (double)top);
+// Over the L lanes of a token.
+template <int L>
+__device__ __forceinline__ float token_max(float v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  }
+  for (int o = L / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, o));
+  return v;
+}
+template <int L>
+__device__ __forceinline__ float token_sum(float v) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+template <int L>
+__device__ __forceinline__ uint32_t token_top(uint32_t v) {
+  if constexpr (L == 32) return __reduce_max_sync(kAll, v);
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(kAll, v, o));
+  return v;
+}
+// The token's lanes for which `yes`, lane 0 of the token in bit 0.
+template <int L>
+__device__ __forceinline__ uint32_t token_lanes(bool yes) {
+  const uint32_t all = __ballot_sync(kAll, yes);
+  return L == 32 ? all : (all >> ((threadIdx.x & 31) / L * L)) & ((1u << (L & 31)) - 1u);
+}
+// Largest two of two descending pairs.
+__device__ __forceinline__ void merge_two(float& first, float& second, float a, float b) {
+  second = fmaxf(fminf(first, a), fmaxf(second, b));
+  first = fmaxf(first, a);
+}
+
+// A token's c in 64 bits to `scratch`, by a whole warp.
+template <typename T>
+__device__ __forceinline__ void scores_again(const RouteParams& p, const T* row, float top, double* scratch) {
+  const int lane = threadIdx.x & 31;
+  double sum = 0.0;
+#pragma unroll 4
   for (int e = lane; e < p.experts; e += 32) {
-    const double v = (double)to_float<T>(row[e]);
-    double c = p.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - (double)top) / sum;
+    const float z = to_float<T>(row[e]);
+    const double s = exp(p.sigmoid ? -(double)z : (double)z - (double)top);
+    sum += s;
+    scratch[e] = s;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
+#pragma unroll 4
+  for (int e = lane; e < p.experts; e += 32) {
+    const double s = scratch[e];
+    double c = p.sigmoid ? 1.0 / (1.0 + s) : s / sum;
     if (p.bias != nullptr) c += (double)p.bias[e];
-    scratch[e] = v == -(double)INFINITY ? v : c;
+    scratch[e] = to_float<T>(row[e]) == -INFINITY ? -(double)INFINITY : c;
   }
   __syncwarp();
-  uint32_t kept = 0xffffffffu;
-  if (p.groups > 1) {
-    unsigned long long mine = 0;
-    if (lane < p.groups) {
-      double first = -(double)INFINITY, second = first;
-      bool bad = false;
-      for (int i = 0; i < size; ++i) {
-        const double c = scratch[lane * size + i];
-        bad |= c != c;
-        if (c > first) {
-          second = first;
-          first = c;
-        } else if (c > second) {
-          second = c;
-        }
+}
+
+// The groups that a token is chosen from, as bits, by their c in 64 bits.
+template <typename T>
+__device__ __noinline__ uint32_t choose_groups_again(const RouteParams& p, const T* row, float top, double* scratch) {
+  const int lane = threadIdx.x & 31, size = p.experts / p.groups;
+  scores_again<T>(p, row, top, scratch);
+  int lanes = 32;  // of a group
+  while (lanes * p.groups > 32) lanes >>= 1;
+  const int group = lane / lanes;
+  double first = -(double)INFINITY, second = first;
+  int bad = 0;
+  if (group < p.groups) {
+    for (int i = lane % lanes; i < size; i += lanes) {
+      const double c = scratch[group * size + i];
+      bad |= c != c;
+      if (c > first) {
+        second = first;
+        first = c;
+      } else if (c > second) {
+        second = c;
       }
-      mine = bad ? 1ull : order_key(p.group_best == 2 ? first + second : first);
-    }
-    kept = 0;
-    for (int j = 0; j < p.top_groups; ++j) {
-      const unsigned long long best = warp_top(mine);
-      const int g = (int)__reduce_min_sync(0xffffffffu, mine == best ? (uint32_t)lane : 32u);
-      kept |= 1u << g;
-      if (lane == g) mine = 0;
     }
   }
+  for (int o = 1; o < lanes; o <<= 1) {
+    const double a = __shfl_xor_sync(kAll, first, o), b = __shfl_xor_sync(kAll, second, o);
+    bad |= __shfl_xor_sync(kAll, bad, o);
+    second = a > first ? (first > b ? first : b) : (second > a ? second : a);
+    first = a > first ? a : first;
+  }
+  const unsigned long long mine = bad ? 1ull : order_key(p.group_best == 2 ? first + second : first);
+  int rank = 0;
+  for (int g = 0; g < p.groups; ++g) {
+    const unsigned long long other = __shfl_sync(kAll, mine, g * lanes);
+    rank += other > mine || (other == mine && g < group);
+  }
+  const bool taken = group < p.groups && lane % lanes == 0 && rank < p.top_groups;
+  const uint32_t kept = __reduce_or_sync(kAll, taken ? 1u << group : 0u);
+  __syncwarp();
+  return kept;
+}
+
+// A token's choice from the groups `kept`, all in 64 bits.
+template <typename T>
+__device__ __noinline__ void choose_again(const RouteParams& p, const T* row, float top, uint32_t kept, double* scratch, int* ids) {
+  const int lane = threadIdx.x & 31, size = p.experts / p.groups;
+  scores_again<T>(p, row, top, scratch);
   for (int j = 0; j < p.top_k; ++j) {
     unsigned long long mine = 0;
-    int at = 0;
+    int at = 0x7fffffff;
     for (int e = lane; e < p.experts; e += 32) {
       if (!((kept >> (p.groups > 1 ? e / size : 0)) & 1u)) continue;
       const double c = scratch[e];
@@ -109,191 +163,366 @@ __device__ __noinline__ void choose_again(const RouteParams& p, const T* row, fl
         at = e;
       }
     }
-    const unsigned long long best = warp_top(mine);
-    const int e = (int)__reduce_min_sync(0xffffffffu, mine == best ? (uint32_t)at : 0x7fffffffu);
-    if (lane == 0) chosen[j] = e;
+    unsigned long long best = mine;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const unsigned long long other = __shfl_xor_sync(kAll, best, o);
+      best = other > best ? other : best;
+    }
+    const int e = (int)__reduce_min_sync(kAll, mine == best ? (uint32_t)at : 0x7fffffffu);
+    if (lane == 0) ids[j] = e;
     if ((e & 31) == lane) scratch[e] = __longlong_as_double(0x7ff8000000000001ll);
     __syncwarp();
   }
 }
 
-// Bound by HBM for many tokens (a logit is read once) and by the chain of maxima for few.
-template <typename T, int V>
+// Orders the first `count` (at most 32) entries of `ids` by their c in 64 bits, by a whole warp; the first top_k are the choice.
+template <typename T>
+__device__ __noinline__ void order_candidates(const RouteParams& p, const T* row, float top, int count, int* ids) {
+  const int lane = threadIdx.x & 31;
+  double sum = 0.0;
+  if (!p.sigmoid) {
+#pragma unroll 4
+    for (int e = lane; e < p.experts; e += 32) sum += exp((double)to_float<T>(row[e]) - (double)top);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
+  }
+  const int e = lane < count ? ids[lane] : 0;
+  unsigned long long mine = 0;
+  if (lane < count) {
+    const double z = (double)to_float<T>(row[e]);
+    double c = p.sigmoid ? 1.0 / (1.0 + exp(-z)) : exp(z - (double)top) / sum;
+    if (p.bias != nullptr) c += (double)p.bias[e];
+    mine = order_key(z == -(double)INFINITY ? z : c);
+  }
+  int rank = 0;
+  for (int j = 0; j < count; ++j) {
+    const unsigned long long other = __shfl_sync(kAll, mine, j);
+    const int other_e = __shfl_sync(kAll, e, j);
+    rank += other > mine || (other == mine && other_e < e);
+  }
+  __syncwarp();
+  if (lane < count) ids[rank] = e;
+  __syncwarp();
+}
+
+// Descending by (key, low).
+template <int V>
+__device__ __forceinline__ void sort_run(uint32_t (&key)[V], uint32_t (&low)[V]) {
+#pragma unroll
+  for (int p = 1; p < V; p <<= 1) {
+#pragma unroll
+    for (int k = p; k >= 1; k >>= 1) {
+#pragma unroll
+      for (int j = k % p; j + k < V; j += 2 * k) {
+#pragma unroll
+        for (int i = 0; i < k; ++i) {
+          if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const int a = i + j, b = i + j + k;
+            const bool swap = key[b] > key[a] || (key[b] == key[a] && low[b] > low[a]);
+            const uint32_t ka = key[a], la = low[a];
+            key[a] = swap ? key[b] : ka;
+            low[a] = swap ? low[b] : la;
+            key[b] = swap ? ka : key[b];
+            low[b] = swap ? la : low[b];
+          }
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int L, int V, bool kByLogit>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteParams p) {
-  extern __shared__ double scratch_all[];  // groups or a bias: the row's c, [warp][32 V]
-  __shared__ int chosen_all[kRouteWarps][32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int size = p.experts / p.groups;
-  const bool by_logit = p.bias == nullptr && (p.groups == 1 || p.group_best == 1);
-  const bool whole_sum = !p.sigmoid && (!p.renormalize || !by_logit);
-  double* scratch = scratch_all + warp * 32 * V;
+  constexpr int kTokens = 32 / L;  // of a warp
+  extern __shared__ double scratch_all[];  // groups or a bias: a row's c, [warp][L V]
+  __shared__ int chosen_all[kRouteWarps][kTokens][32];
+  __shared__ float group_all[kRouteWarps][kTokens][2][32];  // score, magnitude
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, own = lane / L, l = lane % L;
+  const int size = p.experts / p.groups, e0 = l * V;
+  const bool whole_sum = !p.sigmoid && (!p.renormalize || !kByLogit);
+  // Groups of whole lanes, in a power of two of them, find their best by shuffles.
+  const int group_lanes = size % V == 0 && ((size / V) & (size / V - 1)) == 0 ? size / V : 0;
+  double* scratch = scratch_all + (p.groups > 1 || !kByLogit ? warp * L * V : 0);
   float* row_c = reinterpret_cast<float*>(scratch);
-  int* chosen = chosen_all[warp];
+  int* chosen = chosen_all[warp][own];
+  float *group_score = group_all[warp][own][0], *group_size = group_all[warp][own][1];
   chain_release();
   chain_wait();
-  for (long long t = (long long)blockIdx.x * kRouteWarps + warp; t < p.tokens; t += (long long)gridDim.x * kRouteWarps) {
+  float bias[V];
+  if (!kByLogit) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) bias[i] = p.bias != nullptr && e0 + i < p.experts ? p.bias[e0 + i] : 0.f;
+  }
+  const bool vec = p.experts == L * V && p.ld * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.logits) & 15) == 0;
+  const long long step = (long long)gridDim.x * kRouteWarps * kTokens;
+  for (long long t0 = ((long long)blockIdx.x * kRouteWarps + warp) * kTokens; t0 < p.tokens; t0 += step) {
+    const long long t = t0 + own < p.tokens ? t0 + own : p.tokens - 1;  // lanes without a token take the last one too
     const T* row = reinterpret_cast<const T*>(p.logits) + t * p.ld;
     float z[V];
-    uint32_t key[V];
-    float top = -INFINITY;
+    constexpr int kVec = 16 / (int)sizeof(T) < V ? 16 / (int)sizeof(T) : V;
+    if (vec && kVec * sizeof(T) == 16) {
+#pragma unroll
+      for (int i = 0; i < V; i += kVec) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(row + e0 + i);
+        const T* v = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) z[i + j] = to_float<T>(v[j]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) z[i] = e0 + i < p.experts ? to_float<T>(row[e0 + i]) : -INFINITY;
+    }
     bool bad = false;
+    float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int e = lane + 32 * i;
-      z[i] = e < p.experts ? to_float<T>(row[e]) : -INFINITY;
       bad |= z[i] != z[i];
       top = fmaxf(top, z[i]);
     }
-    bad = __any_sync(0xffffffffu, bad);
-    top = warp_max(top);
+    bad = token_lanes<L>(bad) != 0;
+    top = token_max<L>(top);
     float sum = 0.f;
     if (whole_sum) {
 #pragma unroll
       for (int i = 0; i < V; ++i) sum += z[i] == -INFINITY ? 0.f : expf(z[i] - top);
-      sum = warp_sum(sum);
+      sum = token_sum<L>(sum);
     }
     auto score = [&](float v) {
       if (v == -INFINITY) return 0.f;
       return p.sigmoid ? 1.f / (1.f + expf(-v)) : expf(v - top);  // softmax: not yet divided by the sum
     };
-    bool sure = true;
+    uint32_t key[V], low[V];
+    uint32_t kept = kAll;
+    if (!kByLogit) {
+      // z is c from here on.
+      if (p.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          z[i] = z[i] == -INFINITY ? z[i] : gate_quotient(1.f, gate_denominator(z[i] * -kLog2e)) + bias[i];
+      } else {
+        const float over = 1.f / sum;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float e;
+          asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((z[i] - top) * kLog2e));
+          z[i] = z[i] == -INFINITY ? z[i] : fmaf(e, over, bias[i]);
+        }
+      }
+    }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int e = lane + 32 * i;
-      float c = z[i];
-      if (!by_logit && c != -INFINITY) {
-        c = score(z[i]);
-        if (!p.sigmoid) c = c / sum;
-        if (p.bias != nullptr && e < p.experts) c += p.bias[e];
-      }
-      key[i] = e < p.experts ? order_key(c) : 0u;
-      if (p.groups > 1 && e < p.experts) row_c[e] = c;
+      key[i] = order_key(z[i]);
+      low[i] = V - 1 - i;
     }
     if (p.groups > 1) {
-      __syncwarp();
-      uint32_t mine = 0;
-      float magnitude = 0.f;
-      if (lane < p.groups) {
-        float first = -INFINITY, second = first;
+      const bool two = p.group_best == 2;
+      if (group_lanes > 0) {
+        float first = -INFINITY, second = -INFINITY;
         bool nan = false;
-        for (int i = 0; i < size; ++i) {
-          const float c = row_c[lane * size + i];
-          nan |= c != c;
-          if (c > first) {
-            second = first;
-            first = c;
-          } else if (c > second) {
-            second = c;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          nan |= z[i] != z[i];
+          second = fmaxf(second, fminf(first, z[i]));
+          first = fmaxf(first, z[i]);
+        }
+        for (int o = 1; o < group_lanes; o <<= 1) {
+          const float a = __shfl_xor_sync(kAll, first, o), b = __shfl_xor_sync(kAll, second, o);
+          nan |= __shfl_xor_sync(kAll, (int)nan, o) != 0;
+          merge_two(first, second, a, b);
+        }
+        if (l % group_lanes == 0 && l / group_lanes < p.groups) {
+          group_score[l / group_lanes] = nan ? __uint_as_float(0x7fc00000u) : two ? first + second : first;
+          group_size[l / group_lanes] = fabsf(first) + (two ? fabsf(second) : 0.f);
+        }
+      } else {
+        // One token of the warp after the other through the shared row.
+        for (int s = 0; s < kTokens; ++s) {
+          if (own == s) {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+              if (e0 + i < p.experts) row_c[e0 + i] = z[i];
+          }
+          __syncwarp();
+          if (lane < p.groups) {
+            float first = -INFINITY, second = first;
+            bool nan = false;
+            for (int i = 0; i < size; ++i) {
+              const float c = row_c[lane * size + i];
+              nan |= c != c;
+              second = fmaxf(second, fminf(first, c));
+              first = fmaxf(first, c);
+            }
+            group_all[warp][s][0][lane] = nan ? __uint_as_float(0x7fc00000u) : two ? first + second : first;
+            group_all[warp][s][1][lane] = fabsf(first) + (two ? fabsf(second) : 0.f);
+          }
+          __syncwarp();
+        }
+      }
+      __syncwarp();
+      // Rank of every group; the last one taken and the first one left out have to be clearly apart.
+      kept = 0;
+      float border = INFINITY, border_size = 0.f, next = -INFINITY, next_size = 0.f;
+      bool number = true;
+      for (int g = l; g < p.groups; g += L) {
+        const uint32_t k = order_key(group_score[g]);
+        int rank = 0;
+        for (int o = 0; o < p.groups; ++o) {
+          const uint32_t other = order_key(group_score[o]);
+          rank += other > k || (other == k && o < g);
+        }
+        if (rank < p.top_groups) kept |= 1u << g;
+        number &= k > 1u;
+        if (rank == p.top_groups - 1) border = group_score[g], border_size = group_size[g];
+        if (rank == p.top_groups) next = group_score[g], next_size = group_size[g];
+      }
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) {
+        kept |= __shfl_xor_sync(kAll, kept, o);
+        if (!kByLogit) {
+          border = fminf(border, __shfl_xor_sync(kAll, border, o));
+          next = fmaxf(next, __shfl_xor_sync(kAll, next, o));
+          border_size = fmaxf(border_size, __shfl_xor_sync(kAll, border_size, o));
+          next_size = fmaxf(next_size, __shfl_xor_sync(kAll, next_size, o));
+        }
+      }
+      if (!kByLogit && p.top_groups < p.groups) {
+        const bool sure = token_lanes<L>(!number) == 0 && far_apart(border, next, 1.f + border_size + next_size);
+        uint32_t again = __ballot_sync(kAll, !sure);
+        __syncwarp();
+        while (again != 0) {
+          const int s = (__ffs(again) - 1) / L, from = s * L;
+          again &= ~((L == 32 ? kAll : (1u << (L & 31)) - 1u) << from);
+          const T* which = reinterpret_cast<const T*>(p.logits) + __shfl_sync(kAll, t, from) * p.ld;
+          const uint32_t theirs = choose_groups_again<T>(p, which, __shfl_sync(kAll, top, from), scratch);
+          if (own == s) kept = theirs;
+        }
+      }
+      // V consecutive experts are of one or a few groups.
+      int g = e0 / size, left = size - (e0 - g * size);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (left == 0) {
+          ++g;
+          left = size;
+        }
+        --left;
+        if (e0 + i < p.experts && !((kept >> g) & 1u)) key[i] = 0;
+      }
+      __syncwarp();
+    }
+    if (e0 + V > p.experts) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (e0 + i >= p.experts) key[i] = 0;
+    }
+    sort_run(key, low);
+    // The largest head of the token's lanes; the first lane that has it moves on.
+    auto take = [&](uint32_t& best) {
+      best = token_top<L>(key[0]);
+      const int first = __ffs(token_lanes<L>(key[0] == best)) - 1;
+      const int e = e0 + V - 1 - (int)low[0];
+      if (l == first) {
+#pragma unroll
+        for (int i = 0; i + 1 < V; ++i) {
+          key[i] = key[i + 1];
+          low[i] = low[i + 1];
+        }
+        key[V - 1] = 0;
+      }
+      return L == 32 && kByLogit ? (l == first ? e : -1) : __shfl_sync(kAll, e, own * L + first);
+    };
+    if constexpr (kByLogit) {
+      for (int j = 0; j < p.top_k; ++j) {
+        uint32_t best;
+        const int e = take(best);
+        if (L == 32 ? e >= 0 : l == 0) chosen[j] = e;
+      }
+    } else {
+      uint32_t last = 0;
+      int last_e = 0, count = 0;
+      bool near_ties = false;
+      float least = INFINITY;  // candidates are not below it
+      for (int j = 0; j <= p.top_k || (j < 32 && __any_sync(kAll, near_ties && count == j)); ++j) {
+        uint32_t best;
+        const int e = take(best);
+        if (l == 0 && j < 32) chosen[j] = e;
+        if (best == 0) continue;  // every expert has been taken
+        const float value = key_value(best);
+        if (j > 0 && j <= p.top_k) {
+          const float a = key_value(last);
+          if (!far_apart(a, value, fabsf(a))) {
+            const float za = to_float<T>(row[last_e]), zb = to_float<T>(row[e]);
+            near_ties |= !((za == zb && (p.bias == nullptr || p.bias[last_e] == p.bias[e])) ||
+                           (za == -INFINITY && zb == -INFINITY));
           }
         }
-        mine = nan ? 1u : order_key(p.group_best == 2 ? first + second : first);
-        magnitude = fabsf(first) + (p.group_best == 2 ? fabsf(second) : 0.f);
-      }
-      uint32_t kept = 0, last = 0;
-      float last_magnitude = 0.f;
-      for (int j = 0; j <= p.top_groups && j < p.groups; ++j) {
-        const uint32_t best = warp_top(mine);
-        const int g = (int)__reduce_min_sync(0xffffffffu, mine == best ? (uint32_t)lane : 32u);
-        const float size_now = __shfl_sync(0xffffffffu, magnitude, g);
-        if (j == p.top_groups) {  // the first group left out has to be clearly behind the last one taken
-          sure = by_logit || far_apart(key_value(last), key_value(best), 1.f + last_magnitude + size_now);
-          break;
-        }
-        kept |= 1u << g;
+        if (j == p.top_k - 1) least = value - 2.f * kUncertain * (1.f + fabsf(value));
+        if (count == j && (j < p.top_k || value >= least)) count = j + 1;
         last = best;
-        last_magnitude = size_now;
-        if (lane == g) mine = 0;
+        last_e = e;
       }
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int e = lane + 32 * i;
-        if (e < p.experts && !((kept >> (e / size)) & 1u)) key[i] = 0;
-      }
+      // More candidates than are held, or values that are no numbers: all over again.
+      const bool all_again = near_ties && (count >= 32 || !(least == least));
+      uint32_t again = __ballot_sync(kAll, near_ties);
       __syncwarp();
-    }
-    float my_score = 0.f, total = 0.f;  // lane j: the j-th choice
-    uint32_t before = 0;
-    float before_z = 0.f, before_b = 0.f;
-    int my_id = 0;
-    const int picks = by_logit ? p.top_k : p.top_k + 1;  // one more, to know how far it is behind
-    for (int j = 0; j < picks && sure; ++j) {
-      uint32_t mine = 0;
-      int at = 0;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if (key[i] > mine) {
-          mine = key[i];
-          at = lane + 32 * i;
-        }
-      }
-      const uint32_t best = warp_top(mine);
-      if (best == 0) break;  // every expert has been taken
-      const int e = (int)__reduce_min_sync(0xffffffffu, mine == best ? (uint32_t)at : 0x7fffffffu);
-      float v = 0.f;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if (lane + 32 * i == e) {
-          v = z[i];
-          key[i] = 0;
-        }
-      }
-      v = __shfl_sync(0xffffffffu, v, e & 31);
-      if (!by_logit) {
-        const float b = p.bias != nullptr ? p.bias[e] : 0.f;
-        if (j > 0 && !(v == before_z && b == before_b) && !(v == -INFINITY && before_z == -INFINITY))
-          sure = far_apart(key_value(before), key_value(best), fabsf(key_value(before)));
-        before = best;
-        before_z = v;
-        before_b = b;
-      }
-      if (j < p.top_k && lane == j) {
-        my_id = e;
-        my_score = v;
+      while (again != 0) {
+        const int s = (__ffs(again) - 1) / L, from = s * L;
+        again &= ~((L == 32 ? kAll : (1u << (L & 31)) - 1u) << from);
+        const T* which = reinterpret_cast<const T*>(p.logits) + __shfl_sync(kAll, t, from) * p.ld;
+        const float its_top = __shfl_sync(kAll, top, from);
+        const int candidates = __shfl_sync(kAll, count, from);
+        if (__shfl_sync(kAll, (int)all_again, from))
+          choose_again<T>(p, which, its_top, __shfl_sync(kAll, kept, from), scratch, chosen_all[warp][s]);
+        else
+          order_candidates<T>(p, which, its_top, candidates, chosen_all[warp][s]);
       }
     }
-    if (!sure) {
-      choose_again<T>(p, row, top, scratch, chosen);
-      if (lane < p.top_k) {
-        my_id = chosen[lane];
-        my_score = to_float<T>(row[my_id]);
+    __syncwarp();
+    float total = p.sigmoid ? 1.f : sum;
+    if (p.renormalize) {
+      total = 0.f;
+      for (int j = l; j < p.top_k; j += L) total += score(to_float<T>(row[chosen[j]]));
+      total = token_sum<L>(total);
+    }
+    if (t0 + own < p.tokens) {
+      for (int j = l; j < p.top_k; j += L) {
+        const int e = chosen[j];
+        const float s = score(to_float<T>(row[e]));
+        const float w = total == 0.f ? 0.f : s / total;  // nothing to choose from
+        p.ids[t * p.top_k + j] = e;
+        p.weights[t * p.top_k + j] = bad ? __uint_as_float(0x7fc00000u) : w * p.scale;
       }
-      __syncwarp();
     }
-    my_score = lane < p.top_k ? score(my_score) : 0.f;
-    total = p.renormalize ? warp_sum(my_score) : p.sigmoid ? 1.f : sum;
-    if (lane < p.top_k) {
-      const float w = total == 0.f ? 0.f : my_score / total;  // nothing to choose from
-      p.ids[t * p.top_k + lane] = my_id;
-      p.weights[t * p.top_k + lane] = bad ? __uint_as_float(0x7fc00000u) : w * p.scale;
-    }
+    __syncwarp();  // `chosen` is used again
   }
 }
 
-template <typename T, int V>
+template <typename T, int L, int V, bool kByLogit>
 int launch_route(const RouteParams& p, cudaStream_t stream) {
-  const int smem = p.groups > 1 || p.bias != nullptr ? kRouteWarps * 32 * V * (int)sizeof(double) : 0;
-  static bool configured[64] = {false};
-  int dev = 0;
-  MIE_CUDA(cudaGetDevice(&dev));
-  if (V == 32 && dev >= 0 && dev < 64 && !configured[dev]) {
-    MIE_CUDA(cudaFuncSetAttribute(route_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024));
-    configured[dev] = true;
-  }
-  const long long blocks = ((long long)p.tokens + kRouteWarps - 1) / kRouteWarps, most = 8ll * sm_count();
-  MIE_CUDA(launch_chained(route_kernel<T, V>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(kRouteWarps * 32),
+  const int smem = p.groups > 1 || !kByLogit ? kRouteWarps * L * V * (int)sizeof(double) : 0;
+  const int per_block = kRouteWarps * (32 / L);
+  const long long blocks = ((long long)p.tokens + per_block - 1) / per_block, most = 16ll * sm_count();
+  MIE_CUDA(launch_chained(route_kernel<T, L, V, kByLogit>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(kRouteWarps * 32),
                           (size_t)smem, stream, p));
   MIE_LAUNCH_CHECK("route_kernel");
   return MIE_OK;
 }
 
+template <typename T, bool kByLogit>
+int launch_route(const RouteParams& p, cudaStream_t stream) {
+  if (p.experts <= 32) return launch_route<T, 8, 4, kByLogit>(p, stream);
+  if (p.experts <= 64) return launch_route<T, 8, 8, kByLogit>(p, stream);
+  if (p.experts <= 128) return launch_route<T, 16, 8, kByLogit>(p, stream);
+  if (p.experts <= 256) return launch_route<T, 32, 8, kByLogit>(p, stream);
+  if (p.experts <= 512) return launch_route<T, 32, 16, kByLogit>(p, stream);
+  return launch_route<T, 32, 32, kByLogit>(p, stream);
+}
+
 template <typename T>
 int launch_route(const RouteParams& p, cudaStream_t stream) {
-  if (p.experts <= 32) return launch_route<T, 1>(p, stream);
-  if (p.experts <= 64) return launch_route<T, 2>(p, stream);
-  if (p.experts <= 128) return launch_route<T, 4>(p, stream);
-  if (p.experts <= 256) return launch_route<T, 8>(p, stream);
-  if (p.experts <= 512) return launch_route<T, 16>(p, stream);
-  return launch_route<T, 32>(p, stream);
+  const bool by_logit = p.bias == nullptr && (p.groups == 1 || p.group_best == 1);
+  return by_logit ? launch_route<T, true>(p, stream) : launch_route<T, false>(p, stream);
 }
 
 }  // namespace

@@ -31,7 +31,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scores: str = "softmax", 
         raise ValueError("route_experts takes CUDA logits [tokens, experts] in bf16, fp16 or fp32")
     if scores not in SCORES:
         raise ValueError(f"unknown scores {scores!r}: one of {', '.join(SCORES)}")
-    tokens, experts = (int(v) for v in logits.shape)
+    tokens, experts = logits.shape
     if experts > 1 and logits.stride(1) != 1 or tokens > 1 and logits.stride(0) < experts:
         raise ValueError(f"logits need dense rows that do not overlap, not strides {list(logits.stride())}")
     if bias is not None and (bias.dtype is not torch.float32 or tuple(bias.shape) != (experts,) or
@@ -40,15 +40,15 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scores: str = "softmax", 
     if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
         raise ValueError("route_experts has no gradient")
     device, top_k = logits.device, int(top_k)
-    ids = torch.empty(tokens, max(top_k, 0), dtype=torch.int32, device=device)
-    weights = torch.empty(tokens, max(top_k, 0), dtype=torch.float32, device=device)
+    ids = torch.empty((tokens, max(top_k, 0)), dtype=torch.int32, device=device)
+    weights = torch.empty((tokens, max(top_k, 0)), dtype=torch.float32, device=device)
     if tokens == 0:
         return ids, weights
     with _lib.on_device(device):
         _lib.check(_lib.load().mie_route_experts(
-            _lib.ptr(logits), row_stride(logits), _lib.DTYPE_CODES[logits.dtype], _lib.ptr(bias), SCORES[scores], tokens,
-            experts, top_k, groups, top_groups, group_best, int(renormalize), float(scale), _lib.ptr(ids),
-            _lib.ptr(weights), _lib.stream_arg(device)))
+            logits.data_ptr(), row_stride(logits), _lib.DTYPE_CODES[logits.dtype], None if bias is None else bias.data_ptr(),
+            SCORES[scores], tokens, experts, top_k, groups, top_groups, group_best, int(renormalize), float(scale),
+            ids.data_ptr(), weights.data_ptr(), _lib.stream_arg(device)))
     return ids, weights
 
 
@@ -81,17 +81,18 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate_u
     if weights.requires_grad and torch.is_grad_enabled():
         raise ValueError("weights requires a gradient: this operator has none")
     lib = _lib.load()
-    out = torch.empty(tokens, width, dtype=torch.bfloat16, device=device)
+    out = torch.empty((tokens, width), dtype=torch.bfloat16, device=device)
     if tokens == 0:
         return out
     with _lib.on_device(device):
-        scratch = torch.empty(max(1, lib.mie_expert_scratch_bytes(tokens, top_k, experts, width, ff)), dtype=torch.uint8,
+        scratch = torch.empty(lib.mie_expert_scratch_bytes(tokens, top_k, experts, width, ff), dtype=torch.uint8,
                               device=device)
         _lib.check(lib.mie_expert_mlp(
-            _lib.ptr(x), row_stride(x), _lib.index_arg(ids), _lib.ptr(weights), _lib.ptr(gate_up), row_stride(gate_up, 1),
-            row_stride(gate_up), _lib.ptr(down), row_stride(down, 1), row_stride(down), _lib.ptr(residual),
-            0 if residual is None else row_stride(residual), _lib.ptr(out), width, tokens, top_k, experts, width, ff, code,
-            _lib.ptr(scratch), scratch.numel(), _lib.ptr(status), _lib.stream_arg(device)))
+            x.data_ptr(), row_stride(x), _lib.index_arg(ids), weights.data_ptr(), gate_up.data_ptr(), row_stride(gate_up, 1),
+            row_stride(gate_up), down.data_ptr(), row_stride(down, 1), row_stride(down),
+            None if residual is None else residual.data_ptr(), 0 if residual is None else row_stride(residual),
+            out.data_ptr(), width, tokens, top_k, experts, width, ff, code, scratch.data_ptr(), scratch.numel(),
+            status.data_ptr(), _lib.stream_arg(device)))
     return out
 
 

@@ -73,6 +73,9 @@ def activation_code(name: str | None) -> int:
 def check_rows(name: str, tensor: torch.Tensor, shape: tuple[int, ...], device: torch.device) -> None:
     """A bf16 CUDA tensor of ``shape`` whose rows are dense and do not overlap, and that autograd does not follow."""
 
+    if (tensor.dtype is torch.bfloat16 and tensor.shape == shape and tensor.device == device and tensor.is_cuda
+            and tensor.is_contiguous() and not tensor.requires_grad):
+        return
     if tensor.dtype is not torch.bfloat16 or tuple(tensor.shape) != shape:
         raise ValueError(f"{name} must be bf16 {list(shape)}, not {tensor.dtype} {list(tensor.shape)}")
     if tensor.device != device or device.type != "cuda":
@@ -90,7 +93,8 @@ def check_rows(name: str, tensor: torch.Tensor, shape: tuple[int, ...], device: 
 def row_stride(tensor: torch.Tensor, dim: int = 0) -> int:
     """Stride of a dimension of dense rows; where it has a single entry, that of rows without gaps."""
 
-    return tensor.stride(dim) if tensor.shape[dim] > 1 else math.prod(tensor.shape[dim + 1:])
+    shape = tensor.shape
+    return tensor.stride(dim) if shape[dim] > 1 else math.prod(shape[dim + 1:])
 
 
 def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -116,14 +120,14 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
         check_rows("bias", bias, (2 * n if gated else n,), device)
     if residual is not None:
         check_rows("residual", residual, (rows, n), device)
-    out = torch.empty(rows, n, dtype=torch.bfloat16, device=device)
+    out = torch.empty((rows, n), dtype=torch.bfloat16, device=device)
     if rows == 0:
         return out
     with _lib.on_device(device):
         _lib.check(_lib.load().mie_fused_linear(
-            _lib.ptr(x), row_stride(x), _lib.ptr(weight), row_stride(weight), _lib.ptr(bias), _lib.ptr(residual),
-            0 if residual is None else row_stride(residual), _lib.ptr(out), n, rows, n, k, code, int(gated),
-            _lib.ptr(status), _lib.stream_arg(device)))
+            x.data_ptr(), row_stride(x), weight.data_ptr(), row_stride(weight), None if bias is None else bias.data_ptr(),
+            None if residual is None else residual.data_ptr(), 0 if residual is None else row_stride(residual),
+            out.data_ptr(), n, rows, n, k, code, int(gated), status.data_ptr(), _lib.stream_arg(device)))
     return out
 
 
