@@ -492,7 +492,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(
       constexpr int kLanesPerRow = kRowBytes / 16, kRowsPerStep = 128 / kLanesPerRow;
       const int store_row = (int)(threadIdx.x & 127) / kLanesPerRow, store_part = (int)(threadIdx.x & 127) % kLanesPerRow;
       const int store_channel = channel0 + store_part * 8;
-      const bool vec_store = p.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && store_channel + 8 <= p.n;
+      const bool vec_store = p.ldy % 8 == 0 && p.n % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
       const bool vec_residual = has_residual && p.ldr % 8 == 0 && (reinterpret_cast<uintptr_t>(p.residual) & 15) == 0;
       uint4 held[kChunk / kRowsPerStep];
       auto load_residual = [&](int chunk) {
@@ -630,24 +630,57 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(
         }
         asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(threads_of_group) : "memory");
         // Whole runs of y's rows.  The other buffer takes the next chunk, so that one barrier a chunk is enough.
-        uint4 data[kChunk / kRowsPerStep];
+        if (vec_store) {
+          uint4 data[kChunk / kRowsPerStep];
 #pragma unroll
-        for (int i = 0; i < kChunk / kRowsPerStep; ++i) {
-          const int row = i * kRowsPerStep + store_row;
-          data[i] = *reinterpret_cast<const uint4*>(stage + row * kRowBytes + ((store_part ^ (row & 7)) * 16));
-        }
+          for (int i = 0; i < kChunk / kRowsPerStep; ++i) {
+            const int row = i * kRowsPerStep + store_row;
+            data[i] = *reinterpret_cast<const uint4*>(stage + row * kRowBytes + ((store_part ^ (row & 7)) * 16));
+          }
 #pragma unroll
-        for (int i = 0; i < kChunk / kRowsPerStep; ++i) {
-          const int row = chunk * kChunk + i * kRowsPerStep + store_row;
-          if (row >= t.count || !ok || store_channel >= p.n) continue;
-          uint16_t* dst = reinterpret_cast<uint16_t*>(p.y) + (long long)(t.first + row) * p.ldy + store_channel;
-          if (vec_store) {
-            *reinterpret_cast<uint4*>(dst) = data[i];
-          } else {
-            const uint32_t w[4] = {data[i].x, data[i].y, data[i].z, data[i].w};
+          for (int i = 0; i < kChunk / kRowsPerStep; ++i) {
+            const int row = chunk * kChunk + i * kRowsPerStep + store_row;
+            if (row < t.count && ok && store_channel < p.n)
+              *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.y) + (long long)(t.first + row) * p.ldy + store_channel) =
+                  data[i];
+          }
+        } else {
+          // Rows of any alignment: a warp takes eight of them, a lane whole words of y, the ends by halves.  (Eight halves a
+          // lane, as its 16 bytes hold them, touch every sector of a row eight times.)
+          constexpr int kWords = kCtaChannels / 64, kEach = kChunk / 4;
+          const int valid = p.n - channel0 < kCtaChannels ? p.n - channel0 : kCtaChannels;
+          uint32_t word[kEach][kWords];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (store_channel + j < p.n) dst[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+          for (int i = 0; i < kEach; ++i) {
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) {
+              const int row = quad * kEach + i, c = 2 * (lane + 32 * w);
+              word[i][w] = *reinterpret_cast<const uint32_t*>(stage + row * kRowBytes + (((c >> 3) ^ (row & 7)) * 16) + (c & 7) * 2);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < kEach; ++i) {
+            const int row = chunk * kChunk + quad * kEach + i;
+            uint16_t* dst = reinterpret_cast<uint16_t*>(p.y) + (long long)(t.first + row) * p.ldy + channel0;
+            const int odd = (int)(reinterpret_cast<uintptr_t>(dst) >> 1 & 1);  // words of y begin at the next half
+            const bool in = row < t.count && ok;
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) {
+              const int c = 2 * (lane + 32 * w) + odd;
+              uint32_t v = word[i][w];
+              if (odd) {  // the same for the whole warp
+                if (w == 0 && lane == 0 && in && valid > 0) dst[0] = (uint16_t)v;
+                uint32_t next = __shfl_down_sync(0xffffffffu, v, 1);
+                const uint32_t wrapped = __shfl_sync(0xffffffffu, word[i][w + 1 < kWords ? w + 1 : w], 0);
+                if (lane == 31) next = w + 1 < kWords ? wrapped : 0u;
+                v = v >> 16 | next << 16;
+              }
+              if (!in) continue;
+              if (c + 1 < valid)
+                *reinterpret_cast<uint32_t*>(dst + c) = v;
+              else if (c < valid)
+                dst[c] = (uint16_t)v;
+            }
           }
         }
       }
