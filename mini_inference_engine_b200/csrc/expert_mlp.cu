@@ -280,9 +280,9 @@ int launch_routed_few(const Product& up, const Product& out, FewParams q, cudaSt
   const long long pairs = (long long)rows * q.top_k, most = pairs < q.experts ? pairs : q.experts;
   if (int rc = few_weight_map(&map_w, up, q.experts)) return rc;
   if (int rc = row_map(&map_x, up, rows, BN)) return rc;
-  const int ctas = FewSmem<BN, Few::kUp>::kCtasPerSm;
   if (int rc = launch_few<BN, Few::kUp, true>(map_w, map_x, q, most * q.weight_tiles,
-                                              few_split(most * q.weight_tiles, (up.k + 63) / 64, ctas), stream))
+                                              few_split(most * q.weight_tiles, (up.k + 63) / 64, FewSmem<BN, Few::kUp>::kCtasPerSm), 1,
+                                              stream))
     return rc;
   q.p = out;
   q.weight_tiles = (out.n + 127) / 128;
@@ -292,7 +292,8 @@ int launch_routed_few(const Product& up, const Product& out, FewParams q, cudaSt
   const uint32_t box[3] = {64, (uint32_t)BN, 1};
   if (int rc = cached_operand_map(&map_x, 3, out.x, dims, strides, box)) return rc;
   return launch_few<BN, Few::kDown, false>(map_w, map_x, q, q.weight_tiles,
-                                           few_split(q.weight_tiles, (int)most * ((out.k + 63) / 64), ctas), stream);
+                                           few_split(q.weight_tiles, (int)most * ((out.k + 63) / 64), FewSmem<BN, Few::kDown>::kCtasPerSm), 1,
+                                           stream);
 }
 
 int launch_any(const Product& p, long long tiles, cudaStream_t stream) {

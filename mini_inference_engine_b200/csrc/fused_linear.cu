@@ -6,8 +6,6 @@
 namespace mie {
 namespace {
 
-constexpr int kFewRows = 128;
-
 int launch_any(const Product& p, cudaStream_t stream) {
   const int row_tiles = (p.m + kAnyTile - 1) / kAnyTile;
   MIE_CUDA(launch_chained(product_any_kernel<false>,
@@ -17,22 +15,62 @@ int launch_any(const Product& p, cudaStream_t stream) {
   return MIE_OK;
 }
 
-int launch_dense_wide(const Product& p, cudaStream_t stream) {
+long long few_tiles(const Product& p) { return (p.n + (p.gated ? 63 : 127)) / (p.gated ? 64 : 128); }
+
+// Clocks that a product takes: the choice between the kernels, and of their tiles.  The constants are fits of both kernels
+// over 2 to 512 rows of 1000 x 1024, 2560 x 9728, 4096 x 4096, 6144 x 2048, 8192 x 512, 12288 x 2048 and 19456 x 2560 (the
+// last two gated): fixed parts, clocks of a block of 64 columns where a CTA (or pair) has its SM to itself, and all SMs' bytes
+// a clock from HBM, which the weights come from once.
+constexpr double kHbmBytes = 3400.0;
+
+struct WidePlan {
+  int rows;  // of a tile
+  double clocks;
+};
+WidePlan plan_wide(const Product& p) {
+  // As few rounds, of as short tiles, as take the least time.  A block takes a pair 2 clocks a row by its products, and by its
+  // loads 275 clocks and 1.1 a row, 345 at least.
+  const int channels = p.gated ? 128 : 256, pairs = sm_count() / 2, blocks = (p.k + 63) / 64;
+  const long long weight_tiles = (p.n + channels - 1) / channels;
+  WidePlan best = {0, 0.0};
+  for (int rows = kWideRows; rows >= 32; rows -= 16) {
+    const long long row_tiles = (p.m + rows - 1) / rows, tiles = weight_tiles * row_tiles;
+    const double products = 2.0 * rows, loads = 275.0 + 1.1 * rows, fresh = 32768.0 / (row_tiles < 8 ? row_tiles : 8) / kHbmBytes;
+    const double block = products > loads ? products : loads > 345.0 ? loads : 345.0;
+    const long long full = tiles / pairs, rest = tiles % pairs;
+    double clocks = 9500.0 + full * blocks * (block > fresh * pairs ? block : fresh * pairs);
+    if (rest > 0) clocks += blocks * (block > fresh * rest ? block : fresh * rest);
+    if (best.rows == 0 || clocks < best.clocks) best = {rows, clocks};
+  }
+  return best;
+}
+struct FewPlan {
+  int rows, split;
+  double clocks;
+};
+FewPlan plan_few(const Product& p) {
+  const int rows = p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128, blocks = (p.k + 63) / 64, sms = sm_count();
+  const long long row_tiles = (p.m + rows - 1) / rows, tiles = few_tiles(p) * row_tiles;
+  const int split = few_split(tiles, blocks, 2), own = (blocks + split - 1) / split;
+  const double alone = rows == 16 ? 367.0 : rows == 32 ? 378.0 : rows == 64 ? 487.0 : 627.0;
+  const double both = 2.0 * (16384.0 + 128.0 * rows) / 62.0;  // two CTAs on an SM
+  const double fixed = 8500.0 + 15.0 * rows + (split >= 4 ? 1500.0 : split == 2 ? 800.0 : 0.0);
+  const double fresh = 16384.0 / row_tiles / kHbmBytes;
+  const long long ctas = tiles * split, full = ctas / (2 * sms), rest = ctas % (2 * sms);
+  double clocks = fixed + full * own * (both > fresh * 2 * sms ? both : fresh * 2 * sms);
+  if (rest > 0) {
+    const double last = rest <= sms ? alone : both;
+    clocks += own * (last > fresh * rest ? last : fresh * rest);
+  }
+  return {rows, split, clocks};
+}
+
+int launch_dense_wide(const Product& p, const WidePlan& plan, cudaStream_t stream) {
   WideParams q = {};
   q.p = p;
-  const int channels = p.gated ? 128 : 256, pairs = sm_count() / 2;
+  const int channels = p.gated ? 128 : 256;
   q.weight_tiles = (p.n + channels - 1) / channels;
-  // Rows of a tile: the time is the rounds' number times the rows, below 128 of which the weights' way through shared memory
-  // takes as long.
-  long long best = 0;
-  for (int rows = kWideRows; rows >= 128; rows -= 16) {
-    const long long tiles = (long long)q.weight_tiles * ((p.m + rows - 1) / rows);
-    const long long cost = (tiles + pairs - 1) / pairs * (rows + 16);
-    if (q.tile_rows == 0 || cost < best) {
-      best = cost;
-      q.tile_rows = rows;
-    }
-  }
+  q.tile_rows = plan.rows;
   q.row_tiles = (p.m + q.tile_rows - 1) / q.tile_rows;
   q.band = 8;
   q.x_box = q.tile_rows / 2;
@@ -48,23 +86,21 @@ int launch_dense_wide(const Product& p, cudaStream_t stream) {
 }
 
 template <int BN, bool kGated>
-int launch_dense_few(const Product& p, cudaStream_t stream) {
+int launch_dense_few(const Product& p, int split, cudaStream_t stream) {
   FewParams q = {};
   q.p = p;
-  const long long tiles = (p.n + (kGated ? 63 : 127)) / (kGated ? 64 : 128);
   CUtensorMap map_w, map_x;
   if (int rc = few_weight_map(&map_w, p, 1)) return rc;
   if (int rc = row_map(&map_x, p, p.m, BN)) return rc;
-  return launch_few<BN, Few::kDense, kGated>(map_w, map_x, q, tiles,
-                                             few_split(tiles, (p.k + 63) / 64, FewSmem<BN, Few::kDense>::kCtasPerSm), stream);
+  return launch_few<BN, Few::kDense, kGated>(map_w, map_x, q, few_tiles(p), split, (p.m + BN - 1) / BN, stream);
 }
 
 template <bool kGated>
-int launch_dense_few(const Product& p, cudaStream_t stream) {
-  if (p.m <= 16) return launch_dense_few<16, kGated>(p, stream);
-  if (p.m <= 32) return launch_dense_few<32, kGated>(p, stream);
-  if (p.m <= 64) return launch_dense_few<64, kGated>(p, stream);
-  return launch_dense_few<128, kGated>(p, stream);
+int launch_dense_few(const Product& p, const FewPlan& plan, cudaStream_t stream) {
+  if (plan.rows == 16) return launch_dense_few<16, kGated>(p, plan.split, stream);
+  if (plan.rows == 32) return launch_dense_few<32, kGated>(p, plan.split, stream);
+  if (plan.rows == 64) return launch_dense_few<64, kGated>(p, plan.split, stream);
+  return launch_dense_few<128, kGated>(p, plan.split, stream);
 }
 
 }  // namespace
@@ -90,6 +126,8 @@ extern "C" int mie_fused_linear(const void* x, int64_t ldx, const void* w, int64
   p.m = m, p.n = n, p.k = k;
   p.activation = activation, p.gated = gated != 0, p.status = status;
   if (!wide_takes(p)) return launch_any(p, stream);
-  if (m <= kFewRows) return p.gated ? launch_dense_few<true>(p, stream) : launch_dense_few<false>(p, stream);
-  return launch_dense_wide(p, stream);
+  const WidePlan wide = plan_wide(p);
+  const FewPlan few = plan_few(p);
+  if (wide.clocks < few.clocks) return launch_dense_wide(p, wide, stream);
+  return p.gated ? launch_dense_few<true>(p, few, stream) : launch_dense_few<false>(p, few, stream);
 }

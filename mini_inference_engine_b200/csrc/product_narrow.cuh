@@ -30,9 +30,9 @@ constexpr int kFewPairs = kFewRoutedRows * MIE_MAX_TOP_K;
 template <int BN, Few kKind>
 struct FewSmem {
   static constexpr int kStageBytes = 128 * 128 + BN * 128;
-  static constexpr int kCtasPerSm = BN <= 64 ? 2 : 1;
+  static constexpr int kCtasPerSm = 2;
   static constexpr int kRouting = kKind == Few::kDense ? 0 : kFewPairs * 6 + MIE_MAX_EXPERTS * 2 + 256;
-  static constexpr int kStages = ((kCtasPerSm == 2 ? 110 : 220) * 1024 - kRouting) / kStageBytes;
+  static constexpr int kStages = ((kCtasPerSm == 2 ? 111 : 220) * 1024 - kRouting) / kStageBytes;
   static constexpr int kAcc = kKind == Few::kDown ? 4 : 1;  // accumulators in tensor memory
   static constexpr int kAccColumns = BN < 32 ? 32 : BN;
   static constexpr int kTotal = kStages * kStageBytes + kRouting + (2 * kStages + 2 * kAcc) * 8 + 16 + 1024;
@@ -48,7 +48,7 @@ struct FewParams {
   int top_k, experts, weight_tiles;
 };
 
-// The experts in use, ascending, and the pairs' experts and weights, in shared memory.
+// The experts in use, in the same order for kUp and kDown, and the pairs' experts and weights, in shared memory.
 struct Routing {
   int16_t* used;      // [MIE_MAX_EXPERTS]
   int16_t* expert;    // [rows * top_k], -1: none
@@ -67,6 +67,26 @@ __device__ __forceinline__ Routing routing_at(uint8_t* base) {
 }
 __device__ __forceinline__ int find_routing(const Routing& r, const FewParams& q, bool report) {
   const int pairs = q.p.m * q.top_k, tid = threadIdx.x;
+  if (pairs <= 32) {  // one warp, in the order of the pairs
+    if (tid < 32) {
+      const int row = tid / q.top_k;
+      const long long e = tid < pairs ? q.ids.at(row, tid - row * q.top_k) : -1;
+      const bool valid = e >= 0 && e < q.experts;
+      if (!valid && e != -1 && report) raise_status(q.p.status, MIE_STATUS_BAD_EXPERT);
+      const int expert = valid ? (int)e : -1;
+      const uint32_t same = __match_any_sync(0xffffffffu, expert);
+      const bool first = valid && __ffs(same) - 1 == tid;
+      const uint32_t firsts = __ballot_sync(0xffffffffu, first);
+      if (first) r.used[__popc(firsts & ((1u << tid) - 1u))] = (int16_t)expert;
+      if (tid < pairs) {
+        r.expert[tid] = (int16_t)expert;
+        r.weight[tid] = q.weights[tid];
+      }
+      if (tid == 0) *r.count = __popc(firsts);
+    }
+    __syncthreads();
+    return *r.count;
+  }
   if (tid < 32) r.bitmap[tid] = 0;
   __syncthreads();
   for (int i = tid; i < pairs; i += kFewThreads) {
@@ -95,11 +115,20 @@ __device__ __forceinline__ int find_routing(const Routing& r, const FewParams& q
   return *r.count;
 }
 
+// Four channels of a row from the parked sums of all CTAs, in rank order.
 template <int kSplit>
 __device__ __forceinline__ float4 sum_parts(uint32_t park, int at) {
   float4 part[kSplit];
 #pragma unroll
-  for (int peer = 0; peer < kSplit; ++peer) part[peer] = ld_cluster_f4(park + (uint32_t)at * 4u, (uint32_t)peer);
+  for (int peer = 0; peer < kSplit; ++peer) {
+    if (kSplit == 1)
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(part[0].x), "=f"(part[0].y), "=f"(part[0].z), "=f"(part[0].w)
+                   : "r"(park + (uint32_t)at * 4u)
+                   : "memory");
+    else
+      part[peer] = ld_cluster_f4(park + (uint32_t)at * 4u, (uint32_t)peer);
+  }
   float4 sum = part[0];
 #pragma unroll
   for (int peer = 1; peer < kSplit; ++peer) {
@@ -110,12 +139,77 @@ __device__ __forceinline__ float4 sum_parts(uint32_t park, int at) {
   }
   return sum;
 }
-__device__ __forceinline__ float4 sum_parts(uint32_t park, int at, int split) {
-  return split == 8 ? sum_parts<8>(park, at) : split == 4 ? sum_parts<4>(park, at)
-         : split == 2 ? sum_parts<2>(park, at) : sum_parts<1>(park, at);
+
+// The rows of a tile, finished in units of four channels of a row over all threads of the cluster, several units at a time
+// (one by one the latencies of the sums, the residual and the activation took 5 us of 128 rows).
+template <int BN, Few kKind, bool kGated, int kSplit>
+__device__ __forceinline__ void finish_rows(const FewParams& q, uint32_t park, int rank, int rows, long long to0, int channel0) {
+  constexpr int kFours = kGated ? 16 : 32;
+  constexpr int kBatch = BN == 16 || kSplit == 8 ? 1 : kSplit == 4 ? 2 : 4;
+  const Product& p = q.p;
+  const bool has_residual = kKind != Few::kUp && p.residual != nullptr;
+  const bool vec_residual = has_residual && p.ldr % 4 == 0 && (reinterpret_cast<uintptr_t>(p.residual) & 7) == 0;
+  const bool vec_y = p.ldy % 4 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 7) == 0;
+  const int four = (int)threadIdx.x % kFours, channel = channel0 + four * 4;  // the same for all of a thread's units
+  const int valid = p.n - channel < 4 ? p.n - channel : 4;
+  if (valid <= 0) return;
+  float bias[4] = {0.f, 0.f, 0.f, 0.f}, bias_up[4] = {0.f, 0.f, 0.f, 0.f};
+  if (kKind == Few::kDense && p.bias != nullptr) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j >= valid) break;
+      bias[j] = __bfloat162float(p.bias[channel + j]);
+      if (kGated) bias_up[j] = __bfloat162float(p.bias[p.n + channel + j]);
+    }
+  }
+  constexpr int kStep = 128 / kFours * kSplit;  // rows that the cluster finishes at a time
+  for (int first = rank * (128 / kFours) + (int)threadIdx.x / kFours; first < rows; first += kBatch * kStep) {
+    float v[4 * kBatch], u[kBatch][4], r[kBatch][4];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int row = first + b * kStep < rows ? first + b * kStep : first;
+      const float4 s = sum_parts<kSplit>(park, row * 128 + four * 4);
+      v[4 * b] = s.x + bias[0], v[4 * b + 1] = s.y + bias[1], v[4 * b + 2] = s.z + bias[2], v[4 * b + 3] = s.w + bias[3];
+      if (kGated) {
+        const float4 up = sum_parts<kSplit>(park, row * 128 + 64 + four * 4);
+        u[b][0] = up.x + bias_up[0], u[b][1] = up.y + bias_up[1], u[b][2] = up.z + bias_up[2], u[b][3] = up.w + bias_up[3];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[b][j] = 0.f;
+      if (has_residual) {
+        const __nv_bfloat16* src = p.residual + (to0 + row) * p.ldr + channel;
+        if (vec_residual && valid == 4) {
+          const uint2 raw = *reinterpret_cast<const uint2*>(src);
+          const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
+          const float2 hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
+          r[b][0] = lo.x, r[b][1] = lo.y, r[b][2] = hi.x, r[b][3] = hi.y;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j < valid) r[b][j] = __bfloat162float(src[j]);
+        }
+      }
+    }
+    if (kKind != Few::kDown) activate_all(p.activation, v);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      if (first + b * kStep >= rows) break;
+      float o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = (kGated ? v[4 * b + j] * u[b][j] : v[4 * b + j]) + r[b][j];
+      __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(p.y) + (to0 + first + b * kStep) * p.ldy + channel;
+      if (vec_y && valid == 4) {
+        *reinterpret_cast<uint2*>(y) = make_uint2(Mma16816<__nv_bfloat16>::pack(o[0], o[1]), Mma16816<__nv_bfloat16>::pack(o[2], o[3]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j < valid) y[j] = __float2bfloat16_rn(o[j]);
+      }
+    }
+  }
 }
 
-// grid = (tiles, split), cluster = (1, split).
+// grid = (tiles, split, tiles of rows), cluster = (1, split).
 template <int BN, Few kKind, bool kGated>
 __global__ void __launch_bounds__(kFewThreads, FewSmem<BN, kKind>::kCtasPerSm)
     product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const FewParams q) {
@@ -162,6 +256,7 @@ __global__ void __launch_bounds__(kFewThreads, FewSmem<BN, kKind>::kCtasPerSm)
   if (kKind == Few::kUp) chain_release();
   const int used = kKind == Few::kDense ? 1 : find_routing(routing, q, kKind == Few::kUp);
 
+  const int row0 = kKind == Few::kDense ? (int)blockIdx.z * BN : 0, rows = p.m - row0 < BN ? p.m - row0 : BN;
   const int tile = kKind == Few::kUp ? (int)blockIdx.x % q.weight_tiles : (int)blockIdx.x;
   const int place = kKind == Few::kUp ? (int)blockIdx.x / q.weight_tiles : 0;
   const bool idle = kKind == Few::kUp && place >= used;  // the same for a whole cluster
@@ -207,7 +302,7 @@ __global__ void __launch_bounds__(kFewThreads, FewSmem<BN, kKind>::kCtasPerSm)
           const int unit = at / blocks;
           tma_load_3d(dst, &map_x, &full_bar[s], (at - unit * blocks) * 64, 0, unit);
         } else {
-          tma_load_2d(dst, &map_x, &full_bar[s], at * 64, 0);
+          tma_load_2d(dst, &map_x, &full_bar[s], at * 64, row0);
         }
       }
     }
@@ -267,7 +362,7 @@ __global__ void __launch_bounds__(kFewThreads, FewSmem<BN, kKind>::kCtasPerSm)
             }
           }
         }
-        const uint32_t rows = __ballot_sync(0xffffffffu, sent);
+        const uint32_t sent_rows = __ballot_sync(0xffffffffu, sent);
         if (ok && !warp_wait_bounded(&acc_full[acc], (part / kAcc) & 1u)) {
           ok = false;
           raise_status(p.status, MIE_STATUS_WAIT_TIMEOUT);
@@ -285,7 +380,7 @@ __global__ void __launch_bounds__(kFewThreads, FewSmem<BN, kKind>::kCtasPerSm)
 #pragma unroll
         for (int j = 0; j < BN; ++j) {
           const float f = __shfl_sync(0xffffffffu, factor, j);
-          if ((rows >> j) & 1u) sum[j] = fmaf(f, v[j], sum[j]);
+          if ((sent_rows >> j) & 1u) sum[j] = fmaf(f, v[j], sum[j]);
         }
       }
     } else if (count > 0) {
@@ -309,48 +404,14 @@ __global__ void __launch_bounds__(kFewThreads, FewSmem<BN, kKind>::kCtasPerSm)
   __syncwarp();
   if (kKind == Few::kDown) chain_wait();  // every thread: the residual and y belong to the kernels before as well
   cluster_sync_all();
-  if (warp < 4 && !idle) {
-    // Units of four channels of a row, over all CTAs of the cluster.
-    constexpr int kFours = kGated ? 16 : 32;
+  if (warp < 4 && !idle && ok) {
+    const long long to0 = kKind == Few::kUp ? (long long)place * BN : row0;
     const int channel0 = tile * (kGated ? 64 : 128);
-    for (int i = rank * 128 + (int)threadIdx.x; i < p.m * kFours; i += split * 128) {
-      const int row = i / kFours, four = i % kFours, channel = channel0 + four * 4;
-      const float4 s = sum_parts(park, row * 128 + four * 4, split);
-      float v[4] = {s.x, s.y, s.z, s.w};
-      float u[4] = {1.f, 1.f, 1.f, 1.f};
-      if (kGated) {
-        const float4 up = sum_parts(park, row * 128 + 64 + four * 4, split);
-        u[0] = up.x, u[1] = up.y, u[2] = up.z, u[3] = up.w;
-      }
-      if (channel >= p.n || !ok) continue;
-      const int valid = p.n - channel < 4 ? p.n - channel : 4;
-      if (kKind == Few::kDense && p.bias != nullptr) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (j >= valid) break;
-          v[j] += __bfloat162float(p.bias[channel + j]);
-          if (kGated) u[j] += __bfloat162float(p.bias[p.n + channel + j]);
-        }
-      }
-      if (kKind != Few::kDown) activate_all(p.activation, v);
-      if (kGated) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] *= u[j];
-      }
-      const long long to = kKind == Few::kUp ? (long long)place * BN + row : row;
-      if (kKind != Few::kUp && p.residual != nullptr) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (j < valid) v[j] += __bfloat162float(p.residual[to * p.ldr + channel + j]);
-      }
-      __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(p.y) + to * p.ldy + channel;
-      if (valid == 4 && (reinterpret_cast<uintptr_t>(y) & 7) == 0) {
-        *reinterpret_cast<uint2*>(y) = make_uint2(Mma16816<__nv_bfloat16>::pack(v[0], v[1]), Mma16816<__nv_bfloat16>::pack(v[2], v[3]));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (j < valid) y[j] = __float2bfloat16_rn(v[j]);
-      }
+    switch (split) {
+      case 1: finish_rows<BN, kKind, kGated, 1>(q, park, rank, rows, to0, channel0); break;
+      case 2: finish_rows<BN, kKind, kGated, 2>(q, park, rank, rows, to0, channel0); break;
+      case 4: finish_rows<BN, kKind, kGated, 4>(q, park, rank, rows, to0, channel0); break;
+      default: finish_rows<BN, kKind, kGated, 8>(q, park, rank, rows, to0, channel0); break;
     }
   }
   __syncwarp();
@@ -376,7 +437,7 @@ inline int few_weight_map(CUtensorMap* out, const Product& p, int experts) {
 }
 
 template <int BN, Few kKind, bool kGated>
-int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x, const FewParams& q, long long tiles, int split,
+int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x, const FewParams& q, long long tiles, int split, int row_tiles,
                cudaStream_t stream) {
   using S = FewSmem<BN, kKind>;
   static bool configured[64] = {false};
@@ -388,7 +449,7 @@ int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x, const FewPara
     configured[dev] = true;
   }
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)tiles, (unsigned)split, 1);
+  config.gridDim = dim3((unsigned)tiles, (unsigned)split, (unsigned)row_tiles);
   config.blockDim = dim3(kFewThreads, 1, 1);
   config.dynamicSmemBytes = S::kTotal;
   config.stream = stream;
