@@ -224,13 +224,15 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const CombineParams
   }
 }
 
+constexpr int kMostParts = 320;  // CTAs of a few rows' down product that leave a part of the sums
+
 // Where the parts of the scratch begin.
 struct Scratch {
   long long order, position, tiles, tile_count, hidden, exponents, rows, total;
   Scratch(long long tokens, int top_k, int experts, int width, int ff) {
     const long long pairs = tokens * top_k;
     total = 0;
-    order = take(pairs * 4);
+    order = take((pairs > (width + 127) / 128 ? pairs : (width + 127) / 128) * 4);
     position = take(pairs * 4);
     tiles = take(most_tiles(pairs, experts, kAnyTile) * (long long)sizeof(RowTile));
     tile_count = take(4);
@@ -238,7 +240,9 @@ struct Scratch {
     const long long few = tokens > kFewRoutedRows ? 0 : (pairs < experts ? pairs : experts) * (tokens > 16 ? 32 : 16);
     hidden = take((pairs > few ? pairs : few) * ff * 2);
     exponents = take(pairs * exponent_ld(width));
-    rows = take(pairs * width * 4);
+    // Few rows: the parts of the down product, at most one CTA's an SM or one of every tile.
+    const long long tiles = (width + 127) / 128, parts = tokens > kFewRoutedRows ? 0 : (tiles > kMostParts ? tiles : kMostParts) * 32 * 128 * 4;
+    rows = take(pairs * width * 4 > parts ? pairs * width * 4 : parts);
   }
   long long take(long long bytes) {
     const long long at = total;
@@ -270,6 +274,16 @@ int launch_plan(const PlanParams& plan, cudaStream_t stream) {
   return MIE_OK;
 }
 
+// Parts of a few rows' down product that meet in global memory, 0: it goes by clusters.  16 clusters of eight, a CTA an SM at
+// most, do not keep HBM busy, two CTAs an SM do; but the last one to arrive adds 5 us.  The layer in us, clusters and parts,
+// width 2048 and 128 experts of 768: 1 token 22.6 and 27.9, 4 59.6 and 60.5, 8 84 and 79, 32 160 and 144; where clusters of eight
+// come to two CTAs an SM (width 4096, 8 experts of 2048), 2 tokens 39.9 and 41.9, 32 78.8 and 82.0.
+int few_parts(int width, long long pairs, int cluster) {
+  const int tiles = (width + 127) / 128, ctas = 2 * sm_count() < kMostParts ? 2 * sm_count() : kMostParts, parts = ctas / tiles;
+  if (pairs <= 40 || tiles * cluster >= 1.3 * sm_count() || parts <= cluster) return 0;
+  return parts > 24 ? 24 : parts;
+}
+
 // Few rows: every expert in use for all of them (see product_narrow.cuh).
 template <int BN>
 int launch_routed_few(const Product& up, const Product& out, FewParams q, cudaStream_t stream) {
@@ -277,23 +291,24 @@ int launch_routed_few(const Product& up, const Product& out, FewParams q, cudaSt
   CUtensorMap map_w, map_x;
   q.p = up;
   q.weight_tiles = (up.n + 63) / 64;
+  q.down_tiles = (out.n + 127) / 128;
   const long long pairs = (long long)rows * q.top_k, most = pairs < q.experts ? pairs : q.experts;
-  if (int rc = few_weight_map(&map_w, up, q.experts)) return rc;
+  if (int rc = few_weight_map(&map_w, up, q.experts, 64)) return rc;
   if (int rc = row_map(&map_x, up, rows, BN)) return rc;
-  if (int rc = launch_few<BN, Few::kUp, true>(map_w, map_x, q, most * q.weight_tiles,
-                                              few_split(most * q.weight_tiles, (up.k + 63) / 64, FewSmem<BN, Few::kUp>::kCtasPerSm), 1,
-                                              stream))
+  const long long tiles = most * q.weight_tiles, slots = 2ll * sm_count();
+  const int split = few_split(tiles, (up.k + 63) / 64, 2);
+  if (int rc = launch_few<BN, Few::kUp, true>(map_w, map_x, q, split == 1 && tiles > slots ? slots : tiles, split, 1, stream))
     return rc;
   q.p = out;
-  q.weight_tiles = (out.n + 127) / 128;
-  if (int rc = few_weight_map(&map_w, out, q.experts)) return rc;
+  q.weight_tiles = q.down_tiles;
+  if (int rc = few_weight_map(&map_w, out, q.experts, 128)) return rc;
   const uint64_t dims[3] = {(uint64_t)out.k, (uint64_t)BN, (uint64_t)most};
   const uint64_t strides[2] = {(uint64_t)out.ldx * 2, (uint64_t)out.ldx * 2 * BN};
   const uint32_t box[3] = {64, (uint32_t)BN, 1};
   if (int rc = cached_operand_map(&map_x, 3, out.x, dims, strides, box)) return rc;
-  return launch_few<BN, Few::kDown, false>(map_w, map_x, q, q.weight_tiles,
-                                           few_split(q.weight_tiles, (int)most * ((out.k + 63) / 64), FewSmem<BN, Few::kDown>::kCtasPerSm), 1,
-                                           stream);
+  const int cluster = few_split(q.weight_tiles, (int)most * ((out.k + 63) / 64), 2), parts = few_parts(out.n, pairs, cluster);
+  if (parts == 0) q.parts = nullptr;
+  return launch_few<BN, Few::kDown, false>(map_w, map_x, q, q.weight_tiles, parts > 0 ? parts : cluster, 1, stream);
 }
 
 int launch_any(const Product& p, long long tiles, cudaStream_t stream) {
@@ -359,6 +374,7 @@ extern "C" int mie_expert_mlp(const void* x, int64_t ldx, mie_index_t ids, const
   const bool wide = wide_takes(up) && wide_takes(out) && direct_takes(out);
   if (wide && tokens <= kFewRoutedRows) {
     FewParams few = {};
+    few.parts = (float*)(base + s.rows), few.arrived = order;
     few.ids = IndexView(ids), few.weights = weights, few.top_k = top_k, few.experts = experts;
     up.m = out.m = tokens;
     out.y = y, out.ldy = ldy, out.residual = (const __nv_bfloat16*)residual, out.ldr = ldr;

@@ -90,7 +90,7 @@ int launch_dense_few(const Product& p, int split, cudaStream_t stream) {
   FewParams q = {};
   q.p = p;
   CUtensorMap map_w, map_x;
-  if (int rc = few_weight_map(&map_w, p, 1)) return rc;
+  if (int rc = few_weight_map(&map_w, p, 1, kGated ? 64 : 128)) return rc;
   if (int rc = row_map(&map_x, p, p.m, BN)) return rc;
   return launch_few<BN, Few::kDense, kGated>(map_w, map_x, q, few_tiles(p), split, (p.m + BN - 1) / BN, stream);
 }

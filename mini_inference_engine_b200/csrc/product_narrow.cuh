@@ -1,14 +1,15 @@
 // Products of few rows: the weights are streamed once, 128 rows of them a CTA as the M of a tcgen05 accumulator whose N are the
 // BN rows of x.  Bound by HBM, and by the time from the kernel before to the first weights and from the last weights to the
-// end.  K is cut across a cluster of up to 8 CTAs where the weight has too few tiles to fill the GPU; the parts' sums meet in
-// shared memory, in rank order.
+// end.  Where the weight has too few tiles to fill the GPU, K is cut in parts: across a cluster of up to 8 CTAs, whose sums meet
+// in shared memory, or (kDown) over two CTAs an SM, whose sums meet in global memory, added by the last one to come; in either
+// case in the order of the parts.
 //
 //   kDense  y = act(x W^T + b) + res, gated or not
 //   kUp     routed: every expert that any row is sent to, for all rows: hidden[u][row] = act(G x) * (U x), u the expert's
 //           place among those in use.  Rows of x that are not sent there are computed too (the weights are what counts), not
 //           used.
-//   kDown   routed: y[row] = res + sum_u w[row, u] D_u hidden[u][row].  The sum over the experts is one long K, cut across the
-//           cluster; where an expert ends its part is taken out of tensor memory and added, with its weights, to the rows
+//   kDown   routed: y[row] = res + sum_u w[row, u] D_u hidden[u][row].  The sum over the experts is one long K, cut in parts (see
+//           few_parts); where an expert ends its part is taken out of tensor memory and added, with its weights, to the rows
 //           that are sent there and to no others (an expert's infinities stay with its rows).
 //
 // Which experts are in use every CTA finds out by itself from the ids, a few hundred at most.  kUp lets the kernel after it
@@ -31,13 +32,15 @@ template <int BN, Few kKind>
 struct FewSmem {
   static constexpr int kStageBytes = 128 * 128 + BN * 128;
   static constexpr int kCtasPerSm = 2;
+  static constexpr int kParkBytes = BN * 128 * 4;  // kUp: its own, the others' is the idle ring
   static constexpr int kRouting = kKind == Few::kDense ? 0 : kFewPairs * 6 + MIE_MAX_EXPERTS * 2 + 256;
-  static constexpr int kStages = ((kCtasPerSm == 2 ? 111 : 220) * 1024 - kRouting) / kStageBytes;
-  static constexpr int kAcc = kKind == Few::kDown ? 4 : 1;  // accumulators in tensor memory
+  static constexpr int kExtra = kRouting + (kKind == Few::kUp ? kParkBytes : 0);
+  static constexpr int kStages = (111 * 1024 - kExtra) / kStageBytes;
+  static constexpr int kAcc = kKind == Few::kDown ? 4 : kKind == Few::kUp ? 2 : 1;  // accumulators in tensor memory
   static constexpr int kAccColumns = BN < 32 ? 32 : BN;
-  static constexpr int kTotal = kStages * kStageBytes + kRouting + (2 * kStages + 2 * kAcc) * 8 + 16 + 1024;
-  static_assert(kTotal <= (kCtasPerSm == 2 ? 113 : 227) * 1024, "shared memory of an SM");
-  static_assert(kStages * kStageBytes >= BN * 128 * 4, "the ring also parks the fp32 sums");
+  static constexpr int kTotal = kStages * kStageBytes + kExtra + (2 * kStages + 2 * kAcc) * 8 + 16 + 1024;
+  static_assert(kTotal <= 113 * 1024, "shared memory of an SM");
+  static_assert(kStages * kStageBytes >= kParkBytes, "the ring also parks the fp32 sums");
 };
 
 struct FewParams {
@@ -46,6 +49,9 @@ struct FewParams {
   IndexView ids;  // [rows, top_k]
   const float* weights;
   int top_k, experts, weight_tiles;
+  float* parts;    // kDown: [tiles][split][BN][128], null: the parts are a cluster
+  int* arrived;    // kDown: [tiles], zeroed by kUp
+  int down_tiles;  // kUp: how many those are
 };
 
 // The experts in use, in the same order for kUp and kDown, and the pairs' experts and weights, in shared memory.
@@ -209,7 +215,8 @@ __device__ __forceinline__ void finish_rows(const FewParams& q, uint32_t park, i
   }
 }
 
-// grid = (tiles, split, tiles of rows), cluster = (1, split).
+// grid = (tiles, split, tiles of rows), cluster = (1, split) unless the parts meet in global memory.  Without a split, kUp has as many CTAs as run at once, which go
+// through the tiles of all experts without a pause.
 template <int BN, Few kKind, bool kGated>
 __global__ void __launch_bounds__(kFewThreads, FewSmem<BN, kKind>::kCtasPerSm)
     product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const FewParams q) {
@@ -218,7 +225,9 @@ __global__ void __launch_bounds__(kFewThreads, FewSmem<BN, kKind>::kCtasPerSm)
   constexpr int kTmemColumns = kAcc * S::kAccColumns;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(ring + kStages * S::kStageBytes);
+  uint8_t* park_at = kKind == Few::kUp ? ring + kStages * S::kStageBytes : ring;
+  uint64_t* full_bar =
+      reinterpret_cast<uint64_t*>(ring + kStages * S::kStageBytes + (kKind == Few::kUp ? S::kParkBytes : 0));
   uint64_t* empty_bar = full_bar + kStages;
   uint64_t* acc_full = empty_bar + kStages;
   uint64_t* acc_empty = acc_full + kAcc;
@@ -253,28 +262,41 @@ __global__ void __launch_bounds__(kFewThreads, FewSmem<BN, kKind>::kCtasPerSm)
   // kDown reads the ids and weights ahead of its wait: kUp, whose hidden rows it waits for, has waited for what wrote them.
   if (kKind != Few::kUp) chain_release();
   if (kKind != Few::kDown) chain_wait();
-  if (kKind == Few::kUp) chain_release();
+  if (kKind == Few::kUp) {
+    chain_release();
+    for (int i = (int)(blockIdx.x * kFewThreads + threadIdx.x); i < q.down_tiles; i += (int)gridDim.x * kFewThreads) q.arrived[i] = 0;
+  }
   const int used = kKind == Few::kDense ? 1 : find_routing(routing, q, kKind == Few::kUp);
 
   const int row0 = kKind == Few::kDense ? (int)blockIdx.z * BN : 0, rows = p.m - row0 < BN ? p.m - row0 : BN;
-  const int tile = kKind == Few::kUp ? (int)blockIdx.x % q.weight_tiles : (int)blockIdx.x;
-  const int place = kKind == Few::kUp ? (int)blockIdx.x / q.weight_tiles : 0;
-  const bool idle = kKind == Few::kUp && place >= used;  // the same for a whole cluster
-  const int total = kKind == Few::kDown ? used * blocks : blocks;
-  const int first = idle ? 0 : (int)((long long)total * rank / split);
-  const int count = idle ? 0 : (int)((long long)total * (rank + 1) / split) - first;
-  const int expert = kKind == Few::kUp && !idle ? routing.used[place] : 0;
+  // The CTA's work: units of `blocks` blocks of K, each with an accumulator of its own.  kUp: tiles blockIdx.x, + gridDim.x, ...
+  // of all experts' in use; kDown: the experts in use.
+  int units = 1;
+  if (kKind == Few::kUp) {
+    const int left = used * q.weight_tiles - (int)blockIdx.x;
+    units = left <= 0 ? 0 : (left + (int)gridDim.x - 1) / (int)gridDim.x;
+  }
+  if (kKind == Few::kDown) units = used;
+  const int total = units * blocks;
+  const int first = (int)((long long)total * rank / split);
+  const int count = (int)((long long)total * (rank + 1) / split) - first;
+  auto tile_of = [&](int unit) {
+    return kKind == Few::kUp ? ((int)blockIdx.x + unit * (int)gridDim.x) % q.weight_tiles : (int)blockIdx.x;
+  };
+  auto place_of = [&](int unit) {
+    return kKind == Few::kUp ? ((int)blockIdx.x + unit * (int)gridDim.x) / q.weight_tiles : kKind == Few::kDown ? unit : 0;
+  };
 
   bool ok = true;
-  const uint32_t park = smem_u32(ring);
+  const uint32_t park = smem_u32(park_at);
   if (warp == 4) {
     if (lane == 0) {
       const uint64_t policy = l2_evict_first_policy();  // weights are streamed once per call
       int requested = 0;
       auto request_weights = [&](int i) {
         const int s = i % kStages, at = first + i;
-        const int unit = kKind == Few::kDown ? at / blocks : 0, b = kKind == Few::kDown ? at - unit * blocks : at;
-        const int e = kKind == Few::kDown ? routing.used[unit] : expert;
+        const int unit = kKind == Few::kDense ? 0 : at / blocks, b = at - unit * blocks, tile = tile_of(unit);
+        const int e = kKind == Few::kDense ? 0 : routing.used[place_of(unit)];
         uint8_t* dst = ring + (size_t)s * S::kStageBytes;
         mbar_expect_tx(&full_bar[s], S::kStageBytes);
         if (kGated) {
@@ -298,21 +320,20 @@ __global__ void __launch_bounds__(kFewThreads, FewSmem<BN, kKind>::kCtasPerSm)
           request_weights(i);
         }
         uint8_t* dst = ring + (size_t)s * S::kStageBytes + 128 * 128;
-        if (kKind == Few::kDown) {
-          const int unit = at / blocks;
-          tma_load_3d(dst, &map_x, &full_bar[s], (at - unit * blocks) * 64, 0, unit);
-        } else {
-          tma_load_2d(dst, &map_x, &full_bar[s], at * 64, row0);
-        }
+        const int unit = kKind == Few::kDense ? 0 : at / blocks, b = at - unit * blocks;
+        if (kKind == Few::kDown)
+          tma_load_3d(dst, &map_x, &full_bar[s], b * 64, 0, unit);
+        else
+          tma_load_2d(dst, &map_x, &full_bar[s], b * 64, row0);
       }
     }
     __syncwarp();
   } else if (warp == 5) {
     constexpr uint32_t idesc = instr_desc_bf16(128, BN, 0, 0);
-    int part = 0;  // runs of one expert
+    int part = 0;  // runs of one unit
     for (int i = 0; i < count; ++i) {
       const int s = i % kStages;
-      const int in_unit = kKind == Few::kDown ? (first + i) % blocks : i;
+      const int in_unit = kKind == Few::kDense ? i : (first + i) % blocks;
       const bool opens = i == 0 || in_unit == 0;
       const bool closes = i == count - 1 || in_unit == blocks - 1;
       const int acc = part % kAcc;
@@ -345,10 +366,34 @@ __global__ void __launch_bounds__(kFewThreads, FewSmem<BN, kKind>::kCtasPerSm)
     float sum[BN];
 #pragma unroll
     for (int j = 0; j < BN; ++j) sum[j] = 0.f;
+    auto take = [&](int part, float (&v)[BN]) {
+      const int acc = part % kAcc;
+      if (ok && !warp_wait_bounded(&acc_full[acc], (part / kAcc) & 1u)) {
+        ok = false;
+        raise_status(p.status, MIE_STATUS_WAIT_TIMEOUT);
+      }
+      tc_fence_after();
+      if constexpr (BN >= 32) {
+#pragma unroll
+        for (int c = 0; c < BN; c += 32)
+          tmem_ld32(lane_addr + acc * S::kAccColumns + c, *reinterpret_cast<float(*)[32]>(&v[c]));
+      } else {
+        tmem_ld16(lane_addr + acc * S::kAccColumns, *reinterpret_cast<float(*)[16]>(&v[0]));
+      }
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[acc]);
+    };
+    auto store_sums = [&]() {
+#pragma unroll
+      for (int j = 0; j < BN; ++j)
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(park + (uint32_t)((j * 128 + row) * 4)), "f"(sum[j]) : "memory");
+    };
     if constexpr (kKind == Few::kDown) {
       int part = 0;
       for (int at = first; at < first + count; ++part) {
-        const int unit = at / blocks, acc = part % kAcc;
+        const int unit = at / blocks;
         at = (unit + 1) * blocks;
         // Lane j: the weight of row j for this expert, and whether it is sent there.
         float factor = 0.f;
@@ -363,50 +408,80 @@ __global__ void __launch_bounds__(kFewThreads, FewSmem<BN, kKind>::kCtasPerSm)
           }
         }
         const uint32_t sent_rows = __ballot_sync(0xffffffffu, sent);
-        if (ok && !warp_wait_bounded(&acc_full[acc], (part / kAcc) & 1u)) {
-          ok = false;
-          raise_status(p.status, MIE_STATUS_WAIT_TIMEOUT);
-        }
-        tc_fence_after();
         float v[BN];
-        if constexpr (BN == 32)
-          tmem_ld32(lane_addr + acc * S::kAccColumns, v);
-        else
-          tmem_ld16(lane_addr + acc * S::kAccColumns, v);
-        tmem_ld_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[acc]);
+        take(part, v);
 #pragma unroll
         for (int j = 0; j < BN; ++j) {
           const float f = __shfl_sync(0xffffffffu, factor, j);
           if ((sent_rows >> j) & 1u) sum[j] = fmaf(f, v[j], sum[j]);
         }
       }
-    } else if (count > 0) {
-      ok = warp_wait_bounded(&acc_full[0], 0);
-      if (!ok) raise_status(p.status, MIE_STATUS_WAIT_TIMEOUT);
-      tc_fence_after();
-      if constexpr (BN >= 32) {
-#pragma unroll
-        for (int c = 0; c < BN; c += 32) tmem_ld32(lane_addr + c, *reinterpret_cast<float(*)[32]>(&sum[c]));
-      } else {
-        tmem_ld16(lane_addr, *reinterpret_cast<float(*)[16]>(&sum[0]));
+    } else if (kKind == Few::kUp && split == 1) {
+      for (int unit = 0; unit < units; ++unit) {
+        take(unit, sum);
+        store_sums();
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (ok) finish_rows<BN, kKind, kGated, 1>(q, park, 0, rows, (long long)place_of(unit) * BN, tile_of(unit) * 64);
+        asm volatile("bar.sync 1, 128;" ::: "memory");  // the sums may be written over
       }
-      tmem_ld_wait();
+    } else if (count > 0) {
+      take(0, sum);
     }
-    // The ring is idle: the last MMA has been waited for by every finishing warp (one that gave up stores nothing).
-    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (kKind != Few::kUp || split > 1) {
+      // The ring is idle: every finishing warp has waited for the last MMA (one that gave up stores nothing).
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (kKind == Few::kDown) chain_wait();  // the residual and y belong to the kernels before as well
+      if (kKind != Few::kDown || q.parts == nullptr) {
+        store_sums();
+      } else {
+        // The last of a tile's parts to arrive adds them all up, its own as the others from memory.
+        const int tile = (int)blockIdx.x, parts = split;
+        float* own = q.parts + ((long long)(tile * parts + rank) * BN) * 128 + row;
 #pragma unroll
-    for (int j = 0; j < BN; ++j)
-      asm volatile("st.shared.f32 [%0], %1;" ::"r"(park + (uint32_t)((j * 128 + row) * 4)), "f"(sum[j]) : "memory");
+        for (int j = 0; j < BN; ++j)
+          if (j < rows) __stcg(own + j * 128, sum[j]);
+        __threadfence();
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        int* flag = reinterpret_cast<int*>(park_at);
+        if (threadIdx.x == 0) *flag = atomicAdd(&q.arrived[tile], 1);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        const bool last = *flag == parts - 1;
+        __threadfence();
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (last) {
+#pragma unroll
+          for (int j = 0; j < BN; ++j) sum[j] = 0.f;
+          const float* from = q.parts + (long long)(tile * parts) * BN * 128 + row;
+          // Several parts' loads in flight; added one after the other.
+          constexpr int kAtOnce = BN <= 64 ? 64 / BN : 1;
+          for (int part = 0; part < parts; part += kAtOnce) {
+            float v[kAtOnce][BN];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+#pragma unroll
+              for (int j = 0; j < BN; ++j)
+                v[u][j] = part + u < parts && j < rows ? __ldcg(from + ((long long)(part + u) * BN + j) * 128) : 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+#pragma unroll
+              for (int j = 0; j < BN; ++j) sum[j] += v[u][j];
+            }
+          }
+          store_sums();
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          if (ok) finish_rows<BN, kKind, kGated, 1>(q, park, 0, rows, 0, tile * 128);
+        }
+      }
+    }
   }
   __syncwarp();
-  if (kKind == Few::kDown) chain_wait();  // every thread: the residual and y belong to the kernels before as well
   cluster_sync_all();
-  if (warp < 4 && !idle && ok) {
-    const long long to0 = kKind == Few::kUp ? (long long)place * BN : row0;
-    const int channel0 = tile * (kGated ? 64 : 128);
+  // kDown without an expert in use: the residual.
+  if (warp < 4 && ok &&
+      (kKind == Few::kDense || (kKind == Few::kUp && split > 1 && units > 0) || (kKind == Few::kDown && q.parts == nullptr))) {
+    const long long to0 = kKind == Few::kUp ? (long long)place_of(0) * BN : row0;
+    const int channel0 = tile_of(0) * (kGated ? 64 : 128);
     switch (split) {
       case 1: finish_rows<BN, kKind, kGated, 1>(q, park, rank, rows, to0, channel0); break;
       case 2: finish_rows<BN, kKind, kGated, 2>(q, park, rank, rows, to0, channel0); break;
@@ -428,11 +503,11 @@ __global__ void __launch_bounds__(kFewThreads, FewSmem<BN, kKind>::kCtasPerSm)
 // Host side
 // ---------------------------------------------------------------------------
 // Weight rows [experts][n or 2 n][k]; any row count.
-inline int few_weight_map(CUtensorMap* out, const Product& p, int experts) {
+inline int few_weight_map(CUtensorMap* out, const Product& p, int experts, int box_rows) {
   const uint64_t row = (uint64_t)p.ldw * 2;
   const uint64_t dims[3] = {(uint64_t)p.k, (uint64_t)p.n * (p.gated ? 2 : 1), (uint64_t)experts};
   const uint64_t strides[2] = {row, experts > 1 ? (uint64_t)p.w_expert * 2 : row};
-  const uint32_t box[3] = {64, p.gated ? 64u : 128u, 1};
+  const uint32_t box[3] = {64, (uint32_t)box_rows, 1};
   return cached_operand_map(out, 3, p.w, dims, strides, box);
 }
 
@@ -456,7 +531,7 @@ int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x, const FewPara
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 1;
-  attr[0].val.clusterDim.y = (unsigned)split;
+  attr[0].val.clusterDim.y = kKind == Few::kDown && q.parts != nullptr ? 1u : (unsigned)split;
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
