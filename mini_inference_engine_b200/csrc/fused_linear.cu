@@ -33,12 +33,13 @@ WidePlan plan_wide(const Product& p) {
   const int channels = p.gated ? 128 : 256, pairs = sm_count() / 2, blocks = (p.k + 63) / 64;
   const long long weight_tiles = (p.n + channels - 1) / channels;
   WidePlan best = {0, 0.0};
-  for (int rows = kWideRows; rows >= 32; rows -= 16) {
+  const int most = p.m >= kWideRows ? kWideRows : p.m > 32 ? (p.m + 15) / 16 * 16 : 32;
+  for (int rows = most; rows >= 32; rows -= 16) {
     const long long row_tiles = (p.m + rows - 1) / rows, tiles = weight_tiles * row_tiles;
     const double products = 2.0 * rows, loads = 275.0 + 1.1 * rows, fresh = 32768.0 / (row_tiles < 8 ? row_tiles : 8) / kHbmBytes;
     const double block = products > loads ? products : loads > 345.0 ? loads : 345.0;
     const long long full = tiles / pairs, rest = tiles % pairs;
-    double clocks = 9500.0 + full * blocks * (block > fresh * pairs ? block : fresh * pairs);
+    double clocks = 10500.0 + full * blocks * (block > fresh * pairs ? block : fresh * pairs);
     if (rest > 0) clocks += blocks * (block > fresh * rest ? block : fresh * rest);
     if (best.rows == 0 || clocks < best.clocks) best = {rows, clocks};
   }
