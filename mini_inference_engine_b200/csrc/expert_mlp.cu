@@ -25,6 +25,7 @@ struct PlanParams {
   RowTile* tiles;
   int* tile_count;
   int* status;
+  int dense_ids;  // int32 without gaps, 16-byte aligned
 };
 
 constexpr int kPlanThreads = 1024;
@@ -71,39 +72,82 @@ __device__ __forceinline__ int block_scan_before(int v, int* warp_sums) {
   return before;
 }
 
-// One cluster.  Every CTA counts its part of the pairs by expert in shared memory; a thread per expert adds the parts up, and
-// with the offsets from a scan over the experts the pairs get their places.
+// Four consecutive pairs' experts, -1 for none.
+__device__ __forceinline__ void plan_ids(const PlanParams& p, int i, int end, int (&e)[4]) {
+  if (p.dense_ids && i + 4 <= end) {
+    const int4 v = *reinterpret_cast<const int4*>(reinterpret_cast<const int*>(p.ids.ptr) + i);
+    e[0] = v.x, e[1] = v.y, e[2] = v.z, e[3] = v.w;
+  } else {
+    int row = i / p.top_k, j = i - row * p.top_k;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      long long id = -1;
+      if (i + u < end) id = p.ids.at(row, j);
+      e[u] = id >= 0 && id < p.experts ? (int)id : id == -1 ? -1 : -2;
+      if (++j == p.top_k) {
+        j = 0;
+        ++row;
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    if (e[u] >= p.experts || e[u] < -1) {
+      raise_status(p.status, MIE_STATUS_BAD_EXPERT);
+      e[u] = -1;
+    }
+  }
+}
+
+// One cluster, or one CTA.  Every CTA counts its part of the pairs by expert in shared memory; a thread per expert adds the
+// parts up, and with the offsets from a scan over the experts the pairs get their places.  A pair's place among its expert's in
+// the CTA's part is kept in `position` meanwhile.
 __global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const PlanParams p) {
   __shared__ int count[MIE_MAX_EXPERTS], place[MIE_MAX_EXPERTS], warp_sums[32];
   const uint32_t rank = cluster_rank(), ranks = gridDim.x;
-  const int begin = (int)((long long)p.pairs * rank / ranks), end = (int)((long long)p.pairs * (rank + 1) / ranks);
+  const int fours = (p.pairs + 3) / 4;
+  const int begin = (int)((long long)fours * rank / ranks) * 4, stop = (int)((long long)fours * (rank + 1) / ranks) * 4;
+  const int end = stop < p.pairs ? stop : p.pairs;
   chain_release();
   for (int e = threadIdx.x; e < p.experts; e += kPlanThreads) count[e] = 0;
   __syncthreads();
   chain_wait();
-  // A pair's place among its expert's, in this CTA's part, is kept in `position`.
-  for (int i = begin + threadIdx.x; i < end; i += 4 * kPlanThreads) {
-    long long e[4];
+  constexpr int kHeld = 2;  // fours of a thread whose experts and places stay in registers: pairs up to 8192 a CTA
+  int held_e[kHeld][4], held_at[kHeld][4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int j = i + u * kPlanThreads, row = j / p.top_k;
-      e[u] = j < end ? p.ids.at(row, j - row * p.top_k) : -1;
-    }
+  for (int h = 0; h < kHeld; ++h) {
+    const int i = begin + ((int)threadIdx.x + h * kPlanThreads) * 4;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const bool valid = e[u] >= 0 && e[u] < p.experts;
-      if (!valid && e[u] != -1) raise_status(p.status, MIE_STATUS_BAD_EXPERT);
-      if (i + u * kPlanThreads < end) p.position[i + u * kPlanThreads] = valid ? atomicAdd(&count[e[u]], 1) : -1;
-    }
+    for (int u = 0; u < 4; ++u) held_e[h][u] = -1;
+    if (i < end) plan_ids(p, i, end, held_e[h]);
   }
-  plan_cluster_sync();
+#pragma unroll
+  for (int h = 0; h < kHeld; ++h) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) held_at[h][u] = held_e[h][u] >= 0 ? atomicAdd(&count[held_e[h][u]], 1) : -1;
+  }
+  for (int i = begin + ((int)threadIdx.x + kHeld * kPlanThreads) * 4; i < end; i += kPlanThreads * 4) {
+    int e[4];
+    plan_ids(p, i, end, e);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i + u < end) p.position[i + u] = e[u] >= 0 ? atomicAdd(&count[e[u]], 1) : -1;
+  }
+  if (ranks > 1)
+    plan_cluster_sync();
+  else
+    __syncthreads();
   const int e = threadIdx.x;
   int total = 0, before = 0;
   if (e < p.experts) {
-    for (uint32_t r = 0; r < ranks; ++r) {
-      const int c = ld_cluster_int(&count[e], r);
-      if (r < rank) before += c;
-      total += c;
+    if (ranks == 1) {
+      total = count[e];
+    } else {
+      for (uint32_t r = 0; r < ranks; ++r) {
+        const int c = ld_cluster_int(&count[e], r);
+        if (r < rank) before += c;
+        total += c;
+      }
     }
   }
   const int first = block_scan_before(total, warp_sums);
@@ -121,24 +165,36 @@ __global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const PlanPar
     if (e == kPlanThreads - 1) *p.tile_count = tile + tiles;
   }
   __syncthreads();
-  for (int i = begin + threadIdx.x; i < end; i += 4 * kPlanThreads) {
-    long long expert[4];
-    int within[4];
+#pragma unroll
+  for (int h = 0; h < kHeld; ++h) {
+    const int i = begin + ((int)threadIdx.x + h * kPlanThreads) * 4;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int j = i + u * kPlanThreads, row = j / p.top_k;
-      within[u] = j < end ? p.position[j] : -1;
-      expert[u] = j < end ? p.ids.at(row, j - row * p.top_k) : -1;
+      if (i + u >= end) continue;
+      const int sorted = held_at[h][u] >= 0 ? place[held_e[h][u]] + held_at[h][u] : -1;
+      if (sorted >= 0) p.order[sorted] = i + u;
+      held_at[h][u] = sorted;
     }
+    if (i + 4 <= end) {
+      *reinterpret_cast<int4*>(p.position + i) = make_int4(held_at[h][0], held_at[h][1], held_at[h][2], held_at[h][3]);
+    } else {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (within[u] < 0) continue;
-      const int j = i + u * kPlanThreads, sorted = place[expert[u]] + within[u];
-      p.order[sorted] = j;
-      p.position[j] = sorted;
+      for (int u = 0; u < 4; ++u)
+        if (i + u < end) p.position[i + u] = held_at[h][u];
     }
   }
-  plan_cluster_sync();  // no CTA leaves while another may still read its counts
+  for (int i = begin + ((int)threadIdx.x + kHeld * kPlanThreads) * 4; i < end; i += kPlanThreads * 4) {
+    int expert[4];
+    plan_ids(p, i, end, expert);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (i + u >= end || expert[u] < 0) continue;
+      const int sorted = place[expert[u]] + p.position[i + u];
+      p.order[sorted] = i + u;
+      p.position[i + u] = sorted;
+    }
+  }
+  if (ranks > 1) plan_cluster_sync();  // no CTA leaves while another may still read its counts
 }
 
 struct CombineParams {
@@ -170,19 +226,28 @@ __global__ void __launch_bounds__(256) expert_combine_any_kernel(const CombinePa
   }
 }
 
-// Eight entries a thread, eight pairs' rows in flight; bound by HBM.
+// Eight entries a thread, eight pairs' rows in flight, the next token's positions read ahead; bound by HBM.
 __global__ void __launch_bounds__(256) expert_combine_kernel(const CombineParams p) {
   chain_release();
   const bool vec_y = p.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
   const bool vec_r = p.ldr % 8 == 0 && (reinterpret_cast<uintptr_t>(p.residual) & 15) == 0;
+  const int lane = threadIdx.x & 31, step = gridDim.x * blockDim.y;
   chain_wait();
-  for (long long t = (long long)blockIdx.x * blockDim.y + threadIdx.y; t < p.tokens; t += (long long)gridDim.x * blockDim.y) {
-    for (int c = threadIdx.x * 8; c < p.width; c += blockDim.x * 8) {
+  int t = blockIdx.x * blockDim.y + threadIdx.y;
+  // Lane j of a warp: the j-th position of its token (blockDim.x is a multiple of 32).
+  int next = t < p.tokens && lane < p.top_k ? p.position[(long long)t * p.top_k + lane] : -1;
+  for (; t < p.tokens; t += step) {
+    const int position = next;
+    if (t + step < p.tokens) next = lane < p.top_k ? p.position[(long long)(t + step) * p.top_k + lane] : -1;
+    for (int c0 = 0; c0 < p.width; c0 += blockDim.x * 8) {
+      const int c = c0 + threadIdx.x * 8;
+      const bool in = c < p.width;
+      uint4 residual = make_uint4(0, 0, 0, 0);
       float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (p.residual != nullptr) {
-        const __nv_bfloat16* r = p.residual + t * p.ldr + c;
+      if (p.residual != nullptr && in) {
+        const __nv_bfloat16* r = p.residual + (long long)t * p.ldr + c;
         if (vec_r) {
-          Vec<__nv_bfloat16, 8>::load(r, sum);
+          residual = __ldcs(reinterpret_cast<const uint4*>(r));
         } else {
 #pragma unroll
           for (int n = 0; n < 8; ++n) sum[n] = __bfloat162float(r[n]);
@@ -193,12 +258,21 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const CombineParams
         int exponent[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-          const long long row = j0 + u < p.top_k ? p.position[t * p.top_k + j0 + u] : -1;
+          const int row = j0 + u < 32 ? __shfl_sync(0xffffffffu, position, (j0 + u) & 31) : -1;
           raw[u] = make_uint4(0, 0, 0, 0);
           exponent[u] = 0;
-          if (row >= 0) {
-            raw[u] = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.rows) + row * p.width + c));
-            exponent[u] = p.exponents[row * p.exponent_ld + c / 32];
+          if (row >= 0 && in) {
+            raw[u] = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.rows) + (long long)row * p.width + c));
+            exponent[u] = p.exponents[(long long)row * p.exponent_ld + c / 32];
+          }
+        }
+        if (j0 == 0 && p.residual != nullptr && vec_r) {
+          const uint32_t w[4] = {residual.x, residual.y, residual.z, residual.w};
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[n]));
+            sum[2 * n] = f.x;
+            sum[2 * n + 1] = f.y;
           }
         }
 #pragma unroll
@@ -213,7 +287,8 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const CombineParams
           }
         }
       }
-      __nv_bfloat16* y = p.y + t * p.ldy + c;
+      if (!in) continue;
+      __nv_bfloat16* y = p.y + (long long)t * p.ldy + c;
       if (vec_y) {
         Vec<__nv_bfloat16, 8>::store(y, sum);
       } else {
@@ -383,7 +458,8 @@ extern "C" int mie_expert_mlp(const void* x, int64_t ldx, mie_index_t ids, const
   const int tile_rows = wide ? kWideRows : kAnyTile;
   const long long tiles = s.most_tiles(pairs, experts, tile_rows);
   const PlanParams plan{IndexView(ids), pairs, top_k, experts, tile_rows, order, (int*)(base + s.position), (RowTile*)(base + s.tiles),
-                        (int*)(base + s.tile_count), status};
+                        (int*)(base + s.tile_count), status,
+                        !ids.is64 && ids.stride1 == 1 && ids.stride0 == top_k && (reinterpret_cast<uintptr_t>(ids.ptr) & 15) == 0};
   if (int rc = launch_plan(plan, stream)) return rc;
   if (!wide) {
     out.wide = 1;

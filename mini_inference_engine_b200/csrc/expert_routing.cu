@@ -288,10 +288,6 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
       for (int i = 0; i < V; ++i) sum += z[i] == -INFINITY ? 0.f : expf(z[i] - top);
       sum = token_sum<L>(sum);
     }
-    auto score = [&](float v) {
-      if (v == -INFINITY) return 0.f;
-      return p.sigmoid ? 1.f / (1.f + expf(-v)) : expf(v - top);  // softmax: not yet divided by the sum
-    };
     uint32_t key[V], low[V];
     uint32_t kept = kAll;
     if (!kByLogit) {
@@ -479,16 +475,29 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
       }
     }
     __syncwarp();
-    float total = p.sigmoid ? 1.f : sum;
+    // Over the chosen's sum only their ratios count: softmax goes by the largest of the chosen (all may be far below the row's),
+    // and so does sigmoid where it is exp(z) but for a factor of 1 - 2^-86 and may underflow.
+    float total = p.sigmoid ? 1.f : sum, shift = top;
+    bool ratio = !p.sigmoid;
+    if (p.renormalize) {
+      shift = -INFINITY;
+      for (int j = l; j < p.top_k; j += L) shift = fmaxf(shift, to_float<T>(row[chosen[j]]));
+      shift = token_max<L>(shift);
+      ratio |= shift < -60.f;
+    }
+    auto weight = [&](float v) {
+      if (v == -INFINITY) return 0.f;
+      return ratio ? expf(v - shift) : 1.f / (1.f + expf(-v));
+    };
     if (p.renormalize) {
       total = 0.f;
-      for (int j = l; j < p.top_k; j += L) total += score(to_float<T>(row[chosen[j]]));
+      for (int j = l; j < p.top_k; j += L) total += weight(to_float<T>(row[chosen[j]]));
       total = token_sum<L>(total);
     }
     if (t0 + own < p.tokens) {
       for (int j = l; j < p.top_k; j += L) {
         const int e = chosen[j];
-        const float s = score(to_float<T>(row[e]));
+        const float s = weight(to_float<T>(row[e]));
         const float w = total == 0.f ? 0.f : s / total;  // nothing to choose from
         p.ids[t * p.top_k + j] = e;
         p.weights[t * p.top_k + j] = bad ? __uint_as_float(0x7fc00000u) : w * p.scale;

@@ -129,6 +129,7 @@ extern "C" int mie_fused_linear(const void* x, int64_t ldx, const void* w, int64
   if (!wide_takes(p)) return launch_any(p, stream);
   const WidePlan wide = plan_wide(p);
   const FewPlan few = plan_few(p);
-  if (wide.clocks < few.clocks) return launch_dense_wide(p, wide, stream);
+  // A grid has up to 65535 tiles of rows.
+  if (wide.clocks < few.clocks || (m + few.rows - 1) / few.rows > 65535) return launch_dense_wide(p, wide, stream);
   return p.gated ? launch_dense_few<true>(p, few, stream) : launch_dense_few<false>(p, few, stream);
 }

@@ -29,7 +29,7 @@ def plain_route(logits, top_k, *, scores="softmax", bias=None, groups=1, top_gro
         total = e.sum(axis=1, keepdims=True)
         s = np.where(total > 0, e / np.where(total > 0, total, 1.0), 0.0)
     else:
-        s = 1.0 / (1.0 + np.exp(-z))
+        s = np.where(z >= 0, 1.0, np.exp(np.minimum(z, 0.0))) / (1.0 + np.exp(-np.abs(z)))
     # Without a bias the scores' order is the logits'; 64 bits do not tell large ones apart.
     by_logit = bias is None and (groups == 1 or group_best == 1)
     c = z.copy() if by_logit else s + (0.0 if bias is None else bias.double().cpu().numpy())
@@ -45,6 +45,10 @@ def plain_route(logits, top_k, *, scores="softmax", bias=None, groups=1, top_gro
         ids[t] = sorted(allowed, key=lambda e: (-c[t, e], e))[:top_k]
     w = np.take_along_axis(np.where(z == -np.inf, 0.0, s), ids, axis=1)
     if renormalize:
+        # By logarithms (log sigmoid(z) = min(z, 0) - log(1 + exp(-|z|))): 64 bits, too, underflow at the lowest fp32 logit.
+        log = np.take_along_axis(z if scores == "softmax" else np.minimum(z, 0.0) - np.log1p(np.exp(-np.abs(z))), ids, axis=1)
+        most = log.max(axis=1, keepdims=True)
+        w = np.exp(log - np.where(np.isfinite(most), most, 0.0))
         total = w.sum(axis=1, keepdims=True)
         w = np.where(total > 0, w / np.where(total > 0, total, 1.0), 0.0)
     return ids, w * scale
@@ -143,6 +147,23 @@ def test_masked_experts(device):
                 check_route(logits, 10, scores=scores, bias=b, groups=groups, top_groups=top_groups, group_best=best)
                 check_route(logits, 10, scores=scores, bias=b, groups=groups, top_groups=top_groups, group_best=best,
                             renormalize=False)
+
+
+def test_scores_far_below_one(device):
+    """Weights over the sum of the chosen depend on their ratios, however small the scores are."""
+
+    torch.manual_seed(9)
+    logits = torch.randn(40, 48, device=device)
+    bias = torch.zeros(48, device=device)
+    bias[:16] = 2.0                        # chosen for their bias
+    for shift in (50.0, 70.0, 100.0, 300.0):
+        low = logits.clone()
+        low[:, :16] -= shift               # far below the row's maximum
+        check_route(low, 6, scores="softmax", bias=bias)
+        check_route(low, 6, scores="sigmoid", bias=bias)
+        check_route(logits - shift, 6, scores="sigmoid")
+        check_route(logits - shift, 6, scores="softmax")
+        check_route(low, 6, scores="softmax", bias=bias, renormalize=False)
 
 
 def test_logits_that_are_no_numbers(device):

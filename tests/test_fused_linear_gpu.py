@@ -64,6 +64,17 @@ def test_long_and_wide(m, n, k, gated, device):
     check(m, n, k, "gelu", gated, True, True, device)
 
 
+@pytest.mark.parametrize("m,n,k", [(8_500_000, 8, 8), (70_000, 520, 64), (3, 300_000, 64)])
+def test_more_tiles_than_a_grid_has(m, n, k, device):
+    torch.manual_seed(m)
+    x, w, b, _ = operands(m, n, k, False, True, False, device)
+    status = torch.zeros(1, dtype=torch.int32, device=device)
+    out = fused_linear(x, w, b, activation="relu", status=status)
+    for rows in (slice(0, 300), slice(m // 2, m // 2 + 300), slice(m - 300 if m > 300 else 0, m)):
+        assert_within(out[rows], *exact_fused_linear(x[rows], w, b, "relu", False, None))
+    assert int(status.item()) == 0
+
+
 def test_operands_that_start_anywhere(device):
     """Views whose first entry is off a 16-byte border."""
 
