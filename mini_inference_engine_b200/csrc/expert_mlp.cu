@@ -316,7 +316,7 @@ struct Scratch {
     hidden = take((pairs > few ? pairs : few) * ff * 2);
     exponents = take(pairs * exponent_ld(width));
     // Few rows: the parts of the down product, at most one CTA's an SM or one of every tile.
-    const long long tiles = (width + 127) / 128, parts = tokens > kFewRoutedRows ? 0 : (tiles > kMostParts ? tiles : kMostParts) * 32 * 128 * 4;
+    const long long tiles = (width + 127) / 128, parts = tokens > kFewRoutedRows ? 0 : (tiles > kMostParts ? tiles : kMostParts) * (tokens > 16 ? 32 : 16) * 128 * 4;
     rows = take(pairs * width * 4 > parts ? pairs * width * 4 : parts);
   }
   long long take(long long bytes) {
@@ -419,10 +419,10 @@ extern "C" int mie_expert_mlp(const void* x, int64_t ldx, mie_index_t ids, const
                 "a row is longer than its stride");
   MIE_CHECK_ARG(activation >= MIE_ACT_NONE && activation <= MIE_ACT_RELU, "unknown activation %d", activation);
   const int pairs = tokens * top_k;
+  if (tokens == 0) return MIE_OK;
   const Scratch s(tokens, top_k, experts, width, ff);
   MIE_CHECK_ARG(scratch_bytes >= s.total, "scratch of %lld bytes, %lld needed", (long long)scratch_bytes, s.total);
   MIE_CHECK_ARG((reinterpret_cast<uintptr_t>(scratch) & 255) == 0, "scratch must be 256-byte aligned");
-  if (tokens == 0) return MIE_OK;
   uint8_t* base = (uint8_t*)scratch;
   int* order = (int*)(base + s.order);
 

@@ -3,6 +3,8 @@
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from ... import _lib
@@ -11,6 +13,11 @@ from .linear import activation_code, check_rows, row_stride
 MAX_EXPERTS = 1024  # MIE_MAX_EXPERTS
 MAX_TOP_K = 32      # MIE_MAX_TOP_K
 SCORES = {"softmax": 0, "sigmoid": 1}  # MIE_SCORES_*
+
+
+@functools.lru_cache(maxsize=4096)
+def _scratch_bytes(tokens: int, top_k: int, experts: int, width: int, ff: int) -> int:
+    return int(_lib.load().mie_expert_scratch_bytes(tokens, top_k, experts, width, ff))
 
 
 def route_experts(logits: torch.Tensor, top_k: int, *, scores: str = "softmax", bias: torch.Tensor | None = None,
@@ -80,14 +87,12 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate_u
         raise ValueError(f"weights must be dense fp32 {list(ids.shape)} on the device of x")
     if weights.requires_grad and torch.is_grad_enabled():
         raise ValueError("weights requires a gradient: this operator has none")
-    lib = _lib.load()
     out = torch.empty((tokens, width), dtype=torch.bfloat16, device=device)
     if tokens == 0:
         return out
     with _lib.on_device(device):
-        scratch = torch.empty(lib.mie_expert_scratch_bytes(tokens, top_k, experts, width, ff), dtype=torch.uint8,
-                              device=device)
-        _lib.check(lib.mie_expert_mlp(
+        scratch = torch.empty(_scratch_bytes(tokens, top_k, experts, width, ff), dtype=torch.uint8, device=device)
+        _lib.check(_lib.load().mie_expert_mlp(
             x.data_ptr(), row_stride(x), _lib.index_arg(ids), weights.data_ptr(), gate_up.data_ptr(), row_stride(gate_up, 1),
             row_stride(gate_up), down.data_ptr(), row_stride(down, 1), row_stride(down),
             None if residual is None else residual.data_ptr(), 0 if residual is None else row_stride(residual),
