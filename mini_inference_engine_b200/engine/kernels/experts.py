@@ -8,7 +8,7 @@ import functools
 import torch
 
 from ... import _lib
-from .linear import activation_code, check_rows, row_stride
+from .linear import activation_code, check_rows
 
 MAX_EXPERTS = 1024  # MIE_MAX_EXPERTS
 MAX_TOP_K = 32      # MIE_MAX_TOP_K
@@ -53,7 +53,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scores: str = "softmax", 
         return ids, weights
     with _lib.on_device(device):
         _lib.check(_lib.load().mie_route_experts(
-            logits.data_ptr(), row_stride(logits), _lib.DTYPE_CODES[logits.dtype], None if bias is None else bias.data_ptr(),
+            logits.data_ptr(), logits.stride(0) if tokens > 1 else experts, _lib.DTYPE_CODES[logits.dtype], None if bias is None else bias.data_ptr(),
             SCORES[scores], tokens, experts, top_k, groups, top_groups, group_best, int(renormalize), float(scale),
             ids.data_ptr(), weights.data_ptr(), _lib.stream_arg(device)))
     return ids, weights
@@ -75,11 +75,10 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate_u
     code, device = activation_code(activation), x.device
     (tokens, width), (experts, double_ff, _), top_k = x.shape, gate_up.shape, int(ids.shape[1])
     ff = double_ff // 2
-    check_rows("x", x, (tokens, width), device)
-    check_rows("gate_up", gate_up, (experts, 2 * ff, width), device)
-    check_rows("down", down, (experts, width, ff), device)
-    if residual is not None:
-        check_rows("residual", residual, (tokens, width), device)
+    ldx, _ = check_rows("x", x, (tokens, width), device)
+    gate_up_row, gate_up_expert = check_rows("gate_up", gate_up, (experts, 2 * ff, width), device)
+    down_row, down_expert = check_rows("down", down, (experts, width, ff), device)
+    ldr = 0 if residual is None else check_rows("residual", residual, (tokens, width), device)[0]
     if ids.dtype not in (torch.int32, torch.int64) or ids.shape[0] != tokens or ids.device != device:
         raise ValueError(f"ids must be int32 or int64 [{tokens}, top_k] on the device of x")
     if weights.dtype is not torch.float32 or weights.shape != ids.shape or weights.device != device or \
@@ -93,11 +92,10 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate_u
     with _lib.on_device(device):
         scratch = torch.empty(_scratch_bytes(tokens, top_k, experts, width, ff), dtype=torch.uint8, device=device)
         _lib.check(_lib.load().mie_expert_mlp(
-            x.data_ptr(), row_stride(x), _lib.index_arg(ids), weights.data_ptr(), gate_up.data_ptr(), row_stride(gate_up, 1),
-            row_stride(gate_up), down.data_ptr(), row_stride(down, 1), row_stride(down),
-            None if residual is None else residual.data_ptr(), 0 if residual is None else row_stride(residual),
-            out.data_ptr(), width, tokens, top_k, experts, width, ff, code, scratch.data_ptr(), scratch.numel(),
-            status.data_ptr(), _lib.stream_arg(device)))
+            x.data_ptr(), ldx, _lib.index_arg(ids), weights.data_ptr(), gate_up.data_ptr(), gate_up_row, gate_up_expert,
+            down.data_ptr(), down_row, down_expert, None if residual is None else residual.data_ptr(), ldr, out.data_ptr(),
+            width, tokens, top_k, experts, width, ff, code, scratch.data_ptr(), scratch.numel(), status.data_ptr(),
+            _lib.stream_arg(device)))
     return out
 
 

@@ -4,8 +4,6 @@ and of any number of rows with bias, activation or gate, and residual in the epi
 
 from __future__ import annotations
 
-import math
-
 import torch
 
 from ... import _lib
@@ -70,31 +68,32 @@ def activation_code(name: str | None) -> int:
     return code
 
 
-def check_rows(name: str, tensor: torch.Tensor, shape: tuple[int, ...], device: torch.device) -> None:
-    """A bf16 CUDA tensor of ``shape`` whose rows are dense and do not overlap, and that autograd does not follow."""
+def check_rows(name: str, tensor: torch.Tensor, shape: tuple[int, ...], device: torch.device) -> tuple[int, int]:
+    """A bf16 CUDA tensor of ``shape`` whose rows are dense and do not overlap, and that autograd does not follow.  Returns
+    the strides of a row and, of three dimensions, of a matrix; of dimensions with one entry, those of rows without gaps."""
 
-    if (tensor.dtype is torch.bfloat16 and tensor.shape == shape and tensor.device == device and tensor.is_cuda
-            and tensor.is_contiguous() and not tensor.requires_grad):
-        return
+    width = shape[-1]
+    matrix = width * shape[-2] if len(shape) > 1 else width
+    if (tensor.dtype is torch.bfloat16 and tensor.shape == shape and tensor.is_contiguous() and tensor.device == device
+            and tensor.is_cuda and not tensor.requires_grad):
+        return width, matrix
     if tensor.dtype is not torch.bfloat16 or tuple(tensor.shape) != shape:
         raise ValueError(f"{name} must be bf16 {list(shape)}, not {tensor.dtype} {list(tensor.shape)}")
     if tensor.device != device or device.type != "cuda":
         raise ValueError(f"{name} must be on the CUDA device of the other operands, not {tensor.device}")
     if tensor.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: this operator has none")
-    dense, extent = shape[-1] == 1 or tensor.stride(-1) == 1, shape[-1]
-    for size, stride in zip(shape[-2::-1], tensor.stride()[-2::-1]):
+    strides = tensor.stride()
+    dense, extent, leading = width == 1 or strides[-1] == 1, width, []
+    for size, stride in zip(shape[-2::-1], strides[-2::-1]):
         if size > 1:
             dense, extent = dense and stride >= extent, stride * size
+            leading.append(stride)
+        else:
+            leading.append(extent)
     if not dense:
-        raise ValueError(f"{name} needs rows that are dense and do not overlap, not strides {list(tensor.stride())}")
-
-
-def row_stride(tensor: torch.Tensor, dim: int = 0) -> int:
-    """Stride of a dimension of dense rows; where it has a single entry, that of rows without gaps."""
-
-    shape = tensor.shape
-    return tensor.stride(dim) if shape[dim] > 1 else math.prod(shape[dim + 1:])
+        raise ValueError(f"{name} needs rows that are dense and do not overlap, not strides {list(strides)}")
+    return leading[0] if leading else width, leading[1] if len(leading) > 1 else matrix
 
 
 def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -107,27 +106,27 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     if x.ndim != 2 or weight.ndim != 2:
         raise ValueError("fused_linear takes rows [rows, k] and a weight [n, k]")
     code, device = activation_code(activation), x.device
-    (rows, k), n = x.shape, int(weight.shape[0])
-    check_rows("x", x, (rows, k), device)
-    check_rows("weight", weight, (n, k), device)
+    rows, k = x.shape
+    n = weight.shape[0]
+    ldx, _ = check_rows("x", x, (rows, k), device)
+    ldw, _ = check_rows("weight", weight, (n, k), device)
+    if bias is not None:
+        check_rows("bias", bias, (n,), device)
     if gated:
         if n % 2:
             raise ValueError(f"a gated weight has as many gates as ups, not {n} rows")
         n //= 2
     if n < 1 or k < 1:
         raise ValueError("fused_linear needs at least one column and one weight row")
-    if bias is not None:
-        check_rows("bias", bias, (2 * n if gated else n,), device)
-    if residual is not None:
-        check_rows("residual", residual, (rows, n), device)
+    ldr = 0 if residual is None else check_rows("residual", residual, (rows, n), device)[0]
     out = torch.empty((rows, n), dtype=torch.bfloat16, device=device)
     if rows == 0:
         return out
     with _lib.on_device(device):
         _lib.check(_lib.load().mie_fused_linear(
-            x.data_ptr(), row_stride(x), weight.data_ptr(), row_stride(weight), None if bias is None else bias.data_ptr(),
-            None if residual is None else residual.data_ptr(), 0 if residual is None else row_stride(residual),
-            out.data_ptr(), n, rows, n, k, code, int(gated), status.data_ptr(), _lib.stream_arg(device)))
+            x.data_ptr(), ldx, weight.data_ptr(), ldw, None if bias is None else bias.data_ptr(),
+            None if residual is None else residual.data_ptr(), ldr, out.data_ptr(), n, rows, n, k, code, gated,
+            status.data_ptr(), _lib.stream_arg(device)))
     return out
 
 
