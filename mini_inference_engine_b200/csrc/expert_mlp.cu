@@ -478,7 +478,7 @@ extern "C" int mie_expert_mlp(const void* x, int64_t ldx, mie_index_t ids, const
   q.weight_tiles = (ff + 127) / 128;
   if (int rc = weight_maps(&maps, up, experts, false)) return rc;
   if (int rc = row_map(&map_x, up, tokens, 1)) return rc;
-  if (int rc = launch_wide<Rows::kUp, true, false>(maps, map_x, q, tiles * q.weight_tiles, stream)) return rc;
+  if (int rc = launch_wide<Rows::kUp, true, false>(maps, map_x, q, tiles * q.weight_tiles, 1, stream)) return rc;
   q.p = out;
   q.weight_tiles = (width + 255) / 256;
   q.x_box = 32;
@@ -486,7 +486,7 @@ extern "C" int mie_expert_mlp(const void* x, int64_t ldx, mie_index_t ids, const
   q.exponent_ld = s.exponent_ld(width);
   if (int rc = weight_maps(&maps, out, experts, true)) return rc;
   if (int rc = row_map(&map_x, out, pairs, q.x_box)) return rc;
-  if (int rc = launch_wide<Rows::kDown, false, true>(maps, map_x, q, tiles * q.weight_tiles, stream)) return rc;
+  if (int rc = launch_wide<Rows::kDown, false, true>(maps, map_x, q, tiles * q.weight_tiles, 1, stream)) return rc;
   const int lanes = width / 8 < 256 ? (width / 8 + 31) / 32 * 32 : 256, rows_per_block = 256 / lanes;
   const long long blocks = ((long long)tokens + rows_per_block - 1) / rows_per_block, most = 16ll * sm_count();
   MIE_CUDA(launch_chained(expert_combine_kernel, dim3((unsigned)(blocks < most ? blocks : most)),

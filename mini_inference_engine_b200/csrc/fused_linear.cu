@@ -23,16 +23,37 @@ long long few_tiles(const Product& p) { return (p.n + (p.gated ? 63 : 127)) / (p
 // a clock from HBM, which the weights come from once.
 constexpr double kHbmBytes = 3400.0;
 
+// How many clusters of `parts` pairs the GPU runs at once.
+int wide_clusters(int parts) {
+  static int cached[64][8] = {{0}};
+  int dev = 0;
+  if (parts < 2 || parts > 7 || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if (cached[dev][parts] == 0) {
+    int n = 0;
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t config = wide_config<Rows::kDense, false, true>(attr, 1, parts, nullptr);
+    config.numAttrs = 1;
+    if (configure_wide<Rows::kDense, false, true>() != MIE_OK ||
+        cudaOccupancyMaxActiveClusters(&n, product_wide_kernel<Rows::kDense, false, true>, &config) != cudaSuccess) {
+      (void)cudaGetLastError();
+      n = 0;
+    }
+    cached[dev][parts] = n > 0 ? n : -1;
+  }
+  return cached[dev][parts] > 0 ? cached[dev][parts] : 0;
+}
+
 struct WidePlan {
-  int rows;  // of a tile
+  int rows, parts;  // of a tile; pairs that share its K
   double clocks;
 };
 WidePlan plan_wide(const Product& p) {
+  const bool direct = direct_takes(p);
   // As few rounds, of as short tiles, as take the least time.  A block takes a pair 2 clocks a row by its products, and by its
   // loads 275 clocks and 1.1 a row, 345 at least.
   const int channels = p.gated ? 128 : 256, pairs = sm_count() / 2, blocks = (p.k + 63) / 64;
   const long long weight_tiles = (p.n + channels - 1) / channels;
-  WidePlan best = {0, 0.0};
+  WidePlan best = {0, 1, 0.0};
   const int most = p.m >= kWideRows ? kWideRows : p.m > 32 ? (p.m + 15) / 16 * 16 : 32;
   for (int rows = most; rows >= 32; rows -= 16) {
     const long long row_tiles = (p.m + rows - 1) / rows, tiles = weight_tiles * row_tiles;
@@ -41,7 +62,14 @@ WidePlan plan_wide(const Product& p) {
     const long long full = tiles / pairs, rest = tiles % pairs;
     double clocks = 10500.0 + full * blocks * (block > fresh * pairs ? block : fresh * pairs);
     if (rest > 0) clocks += blocks * (block > fresh * rest ? block : fresh * rest);
-    if (best.rows == 0 || clocks < best.clocks) best = {rows, clocks};
+    if (best.rows == 0 || clocks < best.clocks) best = {rows, 1, clocks};
+    // A tile's K cut in parts, where all clusters run at once; the sums' way through shared memory takes a part of the rows.
+    for (int parts = 2; direct && parts <= 4 && blocks >= 4 * parts; parts *= 2) {
+      if (tiles * parts > pairs || tiles > wide_clusters(parts)) break;
+      const double own = (blocks + parts - 1) / parts, split = block > fresh * tiles * parts ? block : fresh * tiles * parts;
+      const double time = 10500.0 + 2500.0 + 6.0 * rows + own * split;
+      if (time < best.clocks) best = {rows, parts, time};
+    }
   }
   return best;
 }
@@ -81,9 +109,9 @@ int launch_dense_wide(const Product& p, const WidePlan& plan, cudaStream_t strea
   if (int rc = weight_maps(&maps, p, 1, direct)) return rc;
   if (int rc = row_map(&map_x, p, p.m, q.x_box)) return rc;
   const long long tiles = (long long)q.row_tiles * q.weight_tiles;
-  return p.gated  ? launch_wide<Rows::kDense, true, false>(maps, map_x, q, tiles, stream)
-         : direct ? launch_wide<Rows::kDense, false, true>(maps, map_x, q, tiles, stream)
-                  : launch_wide<Rows::kDense, false, false>(maps, map_x, q, tiles, stream);
+  return p.gated  ? launch_wide<Rows::kDense, true, false>(maps, map_x, q, tiles, 1, stream)
+         : direct ? launch_wide<Rows::kDense, false, true>(maps, map_x, q, tiles, plan.parts, stream)
+                  : launch_wide<Rows::kDense, false, false>(maps, map_x, q, tiles, 1, stream);
 }
 
 template <int BN, bool kGated>

@@ -69,11 +69,11 @@ __device__ __forceinline__ void tmem_relinquish_pair() {
 __device__ __forceinline__ void tmem_dealloc_pair(uint32_t addr, uint32_t cols) {
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
 }
-// Signals the barrier at this address in both CTAs of the pair.
-__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+// Signals the barrier at this address in both CTAs of the pair whose first has cluster rank `leader`.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar, uint32_t leader) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
                    smem_u32(bar)),
-               "h"((uint16_t)3)
+               "h"((uint16_t)(3u << leader))
                : "memory");
 }
 __device__ __forceinline__ void umma_f16_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
@@ -163,11 +163,16 @@ __device__ __forceinline__ WideTile wide_tile(const WideParams& q, int index) {
   }
 }
 
+// Where a finishing warp parks four of the 32 sums that a lane has of a chunk.
+__device__ __forceinline__ int parked(int warp, int chunk, int four, int lane) { return ((warp * 4 + chunk) * 8 + four) * 512 + lane * 16; }
+static_assert(kWideFinishers * 4 * 8 * 512 <= wide_stages<true>() * kWideStageBytes, "the ring parks a tile's sums");
+
 template <Rows kRows, bool kGated, bool kDirect>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(), 1)
+__global__ void __launch_bounds__(wide_threads<kRows>(), 1)
     product_wide_kernel(const __grid_constant__ WeightMaps maps, const __grid_constant__ CUtensorMap map_x, const WideParams q) {
   static_assert(!(kGated && kDirect) && (kRows != Rows::kDown || kDirect), "what there are finishers for");
   constexpr int kWideStages = wide_stages<kDirect>();
+  constexpr bool kSplits = kRows == Rows::kDense && kDirect;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* chunks = ring + kWideStages * kWideStageBytes;  // [2 groups][2][kChunk][256], not kDirect
@@ -178,8 +183,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   const Product& p = q.p;
   const int warp = uniform_warp_index(), lane = threadIdx.x & 31;
+  // grid = (2 pairs, parts), cluster = (2, parts): the pairs of a cluster share the K of one tile.
   const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int blocks = (p.k + 63) / 64;
+  const int part = kSplits ? (int)blockIdx.y : 0, parts = kSplits ? (int)gridDim.y : 1;
+  const uint32_t leader = 2u * (uint32_t)part;  // cluster rank of the pair's first CTA
+  const int all_blocks = (p.k + 63) / 64, block0 = (int)((long long)all_blocks * part / parts);
+  const int blocks = (int)((long long)all_blocks * (part + 1) / parts) - block0;
 
   if (warp == kWideFinishers && lane == 0) {
     for (int s = 0; s < kWideStages; ++s) {
@@ -227,26 +236,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(
           break;
         }
         if (elect_one()) {
-          const uint32_t bar = at_rank(&full_bar[s], 0);
+          const uint32_t bar = at_rank(&full_bar[s], leader);
           if (rank == 0) mbar_expect_tx(&full_bar[s], bytes);
           if constexpr (kGated || kDirect) {
             constexpr int kRun = kGated ? 8 : 32, kRuns = kGated ? 8 : 4, kRunBytes = 16384 / kRuns;
             const int run = (t.weight * 2 + rank) * kRuns, whole = p.n / kRun;
             if (run + kRuns <= whole || whole * kRun == p.n) {
-              tma_pair_5d(dst, &maps.all, bar, b * 64, 0, 0, run, t.expert);
+              tma_pair_5d(dst, &maps.all, bar, (block0 + b) * 64, 0, 0, run, t.expert);
             } else {
               for (int i = 0; i < kRuns; ++i) {
                 if (run + i == whole)
-                  tma_pair_5d(dst + i * kRunBytes, &maps.rest, bar, b * 64, 0, 0, 0, t.expert);
+                  tma_pair_5d(dst + i * kRunBytes, &maps.rest, bar, (block0 + b) * 64, 0, 0, 0, t.expert);
                 else
-                  tma_pair_5d(dst + i * kRunBytes, &maps.run, bar, b * 64, 0, 0, run + i, t.expert);
+                  tma_pair_5d(dst + i * kRunBytes, &maps.run, bar, (block0 + b) * 64, 0, 0, run + i, t.expert);
               }
             }
           } else {
-            tma_pair_3d(dst, &maps.all, bar, b * 64, t.weight * 256 + rank * 128, t.expert);
+            tma_pair_3d(dst, &maps.all, bar, (block0 + b) * 64, t.weight * 256 + rank * 128, t.expert);
           }
           for (int i = 0; i < boxes; ++i)
-            tma_pair_2d(dst + 16384 + (size_t)i * q.x_box * 128, &map_x, bar, b * 64, first + i * q.x_box);
+            tma_pair_2d(dst + 16384 + (size_t)i * q.x_box * 128, &map_x, bar, (block0 + b) * 64, first + i * q.x_box);
         }
         __syncwarp();
       }
@@ -287,7 +296,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(
           break;
         }
         if (elect_one()) {
-          const uint32_t bar = at_rank(&full_bar[s], 0);
+          const uint32_t bar = at_rank(&full_bar[s], leader);
           uint8_t* dst = ring + (size_t)s * kWideStageBytes + 16384 + gatherer * 512;
 #pragma unroll
           for (int i = 0; i < kFours; ++i)
@@ -325,8 +334,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               umma_f16_pair(tmem + acc * 256, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc, b > 0 || k > 0 ? 1u : 0u);
-            umma_commit_pair(&empty_bar[s]);
-            if (b == blocks - 1) umma_commit_pair(&acc_full[acc]);
+            umma_commit_pair(&empty_bar[s], leader);
+            if (b == blocks - 1) umma_commit_pair(&acc_full[acc], leader);
           }
           __syncwarp();
         }
@@ -361,23 +370,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(
             held[i] = *reinterpret_cast<const uint2*>(p.residual + (long long)(t.first + row) * p.ldr + channel);
         }
       };
-      if (has_residual && group < n_chunks) load_residual(group);
-      if (ok && !warp_wait_bounded(&acc_full[acc], (round >> 1) & 1u)) {
-        ok = false;
-        raise_status(p.status, MIE_STATUS_WAIT_TIMEOUT);
-      }
-      tc_fence_after();
-      for (int chunk = group; chunk < n_chunks; chunk += 2) {
-        float v[2][16];  // [j / 2][4 i + 2 (j % 2) + c]
-        const uint32_t from = tmem + (uint32_t)(acc * 256 + chunk * kChunk) + ((uint32_t)(quad * 32) << 16);
-        tmem_ld_fragments(from, v[0]);
-        tmem_ld_fragments(from + (16u << 16), v[1]);
-        tmem_ld_wait();
-        if (chunk + 2 >= n_chunks) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_at(at_rank(&acc_empty[acc], 0));
-        }
+      auto finish = [&](int chunk, float (&v)[2][16]) {  // [j / 2][4 i + 2 (j % 2) + c]
         const int row0 = chunk * kChunk + 2 * pick;
         uint16_t* y = reinterpret_cast<uint16_t*>(p.y) + (long long)(t.first + row0) * p.ldy + channel;
         if constexpr (kRows == Rows::kDown) {
@@ -455,13 +448,66 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(
                     make_uint2(pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]));
             }
           }
+        }
+      };
+      const bool splits = kSplits && parts > 1;  // one tile a cluster
+      if (has_residual && !splits && group < n_chunks) load_residual(group);
+      if (ok && !warp_wait_bounded(&acc_full[acc], (round >> 1) & 1u)) {
+        ok = false;
+        raise_status(p.status, MIE_STATUS_WAIT_TIMEOUT);
+      }
+      tc_fence_after();
+      for (int chunk = group; chunk < n_chunks; chunk += 2) {
+        float v[2][16];
+        const uint32_t from = tmem + (uint32_t)(acc * 256 + chunk * kChunk) + ((uint32_t)(quad * 32) << 16);
+        tmem_ld_fragments(from, v[0]);
+        tmem_ld_fragments(from + (16u << 16), v[1]);
+        tmem_ld_wait();
+        if (chunk + 2 >= n_chunks) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_at(at_rank(&acc_empty[acc], leader));
+        }
+        if (splits) {
+          // The ring is idle: this pair's last MMA is done.
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<float4*>(ring + parked(warp, chunk >> 1, i, lane)) =
+                make_float4(v[i >> 2][4 * (i & 3)], v[i >> 2][4 * (i & 3) + 1], v[i >> 2][4 * (i & 3) + 2], v[i >> 2][4 * (i & 3) + 3]);
+        } else {
+          finish(chunk, v);
           if (has_residual && chunk + 2 < n_chunks) load_residual(chunk + 2);
         }
       }
       if (group >= n_chunks) {  // no chunk of this tile
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_at(at_rank(&acc_empty[acc], 0));
+        if (lane == 0) mbar_arrive_at(at_rank(&acc_empty[acc], leader));
+      }
+      if (splits) {
+        // Every part finishes some of the chunks: the sums of all, in the order of the parts.
+        __syncwarp();
+        cluster_sync_all();
+        for (int chunk = group + 2 * part; chunk < n_chunks; chunk += 2 * parts) {
+          if (has_residual) load_residual(chunk);
+          float v[2][16];
+#pragma unroll
+          for (int f = 0; f < 32; ++f) v[f >> 4][f & 15] = 0.f;
+          for (int other = 0; other < parts; ++other) {
+            float4 a[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              a[i] = ld_cluster_f4(smem_u32(ring + parked(warp, chunk >> 1, i, lane)), 2u * (uint32_t)other + (uint32_t)rank);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              v[i >> 2][4 * (i & 3)] += a[i].x;
+              v[i >> 2][4 * (i & 3) + 1] += a[i].y;
+              v[i >> 2][4 * (i & 3) + 2] += a[i].z;
+              v[i >> 2][4 * (i & 3) + 3] += a[i].w;
+            }
+          }
+          finish(chunk, v);
+        }
       }
     }
   } else {
@@ -547,7 +593,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(
         if (chunk + 2 >= n_chunks) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_at(at_rank(&acc_empty[acc], 0));
+          if (lane == 0) mbar_arrive_at(at_rank(&acc_empty[acc], leader));
           released = true;
         }
         if (has_residual) {
@@ -687,11 +733,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(wide_threads<kRows>(
       if (!released) {  // a group without a chunk of this tile
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_at(at_rank(&acc_empty[acc], 0));
+        if (lane == 0) mbar_arrive_at(at_rank(&acc_empty[acc], leader));
       }
     }
   }
   __syncwarp();
+  if (kSplits && parts > 1 && warp >= kWideFinishers) cluster_sync_all();  // the finishing warps' barrier before they add up
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // no CTA leaves while its barriers or staged rows may be used by the other
@@ -748,18 +795,46 @@ inline bool direct_takes(const Product& p) {
 }
 
 template <Rows kRows, bool kGated, bool kDirect>
-int launch_wide(const WeightMaps& maps, const CUtensorMap& map_x, const WideParams& q, long long most_tiles,
-                cudaStream_t stream) {
+cudaLaunchConfig_t wide_config(cudaLaunchAttribute (&attr)[2], int pairs, int parts, cudaStream_t stream) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)(2 * pairs), (unsigned)parts);
+  config.blockDim = dim3(wide_threads<kRows>());
+  config.dynamicSmemBytes = wide_smem<kDirect>();
+  config.stream = stream;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = (unsigned)parts;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = chained_launch_enabled() ? 2 : 1;
+  return config;
+}
+
+template <Rows kRows, bool kGated, bool kDirect>
+int configure_wide() {
   static bool configured[64] = {false};
   int dev = 0;
   MIE_CUDA(cudaGetDevice(&dev));
-  if (dev >= 0 && dev < 64 && !configured[dev]) {
-    MIE_CUDA(cudaFuncSetAttribute(product_wide_kernel<kRows, kGated, kDirect>, cudaFuncAttributeMaxDynamicSharedMemorySize, wide_smem<kDirect>()));
-    configured[dev] = true;
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    MIE_CUDA(cudaFuncSetAttribute(product_wide_kernel<kRows, kGated, kDirect>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  wide_smem<kDirect>()));
+    if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  const long long most = sm_count() / 2;
-  MIE_CUDA(launch_chained(product_wide_kernel<kRows, kGated, kDirect>, dim3((unsigned)(2 * (most_tiles < most ? most_tiles : most))),
-                          dim3(wide_threads<kRows>()), wide_smem<kDirect>(), stream, maps, map_x, q));
+  return MIE_OK;
+}
+
+// `parts` pairs share a tile's K (kDense, kDirect); then there are as many tiles as pairs.
+template <Rows kRows, bool kGated, bool kDirect>
+int launch_wide(const WeightMaps& maps, const CUtensorMap& map_x, const WideParams& q, long long most_tiles, int parts,
+                cudaStream_t stream) {
+  if (int rc = configure_wide<kRows, kGated, kDirect>()) return rc;
+  const long long most = parts > 1 ? most_tiles : sm_count() / 2;
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t config = wide_config<kRows, kGated, kDirect>(attr, (int)(most_tiles < most ? most_tiles : most), parts, stream);
+  prefer_shared_carveout(reinterpret_cast<const void*>(product_wide_kernel<kRows, kGated, kDirect>));
+  MIE_CUDA(cudaLaunchKernelEx(&config, product_wide_kernel<kRows, kGated, kDirect>, maps, map_x, q));
   MIE_LAUNCH_CHECK("product_wide_kernel");
   return MIE_OK;
 }

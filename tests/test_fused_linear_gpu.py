@@ -59,7 +59,9 @@ def test_rows_without_alignment(m, n, k, pad, gated, device):
 
 
 @pytest.mark.parametrize("m,n,k,gated", [(1, 6144, 2048, True), (24, 2560, 9728, False), (3, 256, 12288, False),
-                                         (2048, 1536, 2560, True), (1021, 5003, 2056, False), (128, 12288, 512, True)])
+                                         (2048, 1536, 2560, True), (1021, 5003, 2056, False), (128, 12288, 512, True),
+                                         (256, 2560, 9728, False), (130, 1000, 4096, False), (400, 4096, 4096, False),
+                                         (161, 2052, 2104, False), (300, 768, 3000, False), (512, 520, 8192, False)])
 def test_long_and_wide(m, n, k, gated, device):
     check(m, n, k, "gelu", gated, True, True, device)
 
