@@ -17,12 +17,6 @@ int launch_any(const Product& p, cudaStream_t stream) {
 
 long long few_tiles(const Product& p) { return (p.n + (p.gated ? 63 : 127)) / (p.gated ? 64 : 128); }
 
-// Clocks that a product takes: the choice between the kernels, and of their tiles.  The constants are fits of both kernels
-// over 2 to 512 rows of 1000 x 1024, 2560 x 9728, 4096 x 4096, 6144 x 2048, 8192 x 512, 12288 x 2048 and 19456 x 2560 (the
-// last two gated): fixed parts, clocks of a block of 64 columns where a CTA (or pair) has its SM to itself, and all SMs' bytes
-// a clock from HBM, which the weights come from once.
-constexpr double kHbmBytes = 3400.0;
-
 // How many clusters of `parts` pairs the GPU runs at once.
 int wide_clusters(int parts) {
   static int cached[64][8] = {{0}};
@@ -43,31 +37,38 @@ int wide_clusters(int parts) {
   return cached[dev][parts] > 0 ? cached[dev][parts] : 0;
 }
 
+// Clocks that a product takes: the choice between the kernels, and of their tiles.  The constants are fits to both kernels'
+// times with every tile and cut, for 1 to 1024 rows of nine weights between 1000 x 1024 and 19456 x 2560 (gated): a fixed part
+// (start, first loads, the last tile's epilogue, and what sums in parts cost), clocks of a block of 64 columns where a CTA or
+// pair has its SMs' loads to itself and where all run, and all SMs' bytes a clock from HBM, which the weights come from once.
+constexpr double kHbmBytes = 3400.0;
+
 struct WidePlan {
   int rows, parts;  // of a tile; pairs that share its K
   double clocks;
 };
 WidePlan plan_wide(const Product& p) {
   const bool direct = direct_takes(p);
-  // As few rounds, of as short tiles, as take the least time.  A block takes a pair 2 clocks a row by its products, and by its
-  // loads 275 clocks and 1.1 a row, 345 at least.
   const int channels = p.gated ? 128 : 256, pairs = sm_count() / 2, blocks = (p.k + 63) / 64;
   const long long weight_tiles = (p.n + channels - 1) / channels;
   WidePlan best = {0, 1, 0.0};
   const int most = p.m >= kWideRows ? kWideRows : p.m > 32 ? (p.m + 15) / 16 * 16 : 32;
   for (int rows = most; rows >= 32; rows -= 16) {
     const long long row_tiles = (p.m + rows - 1) / rows, tiles = weight_tiles * row_tiles;
-    const double products = 2.0 * rows, loads = 275.0 + 1.1 * rows, fresh = 32768.0 / (row_tiles < 8 ? row_tiles : 8) / kHbmBytes;
-    const double block = products > loads ? products : loads > 345.0 ? loads : 345.0;
+    const double fresh = 32768.0 / (row_tiles < 8 ? row_tiles : 8) / kHbmBytes;
+    const double few = 380.0 + 0.2 * rows > 2.36 * rows + 6.0 ? 380.0 + 0.2 * rows : 2.36 * rows + 6.0;
+    const double all = 241.0 + 1.61 * rows > 390.0 ? 241.0 + 1.61 * rows : 390.0;
     const long long full = tiles / pairs, rest = tiles % pairs;
-    double clocks = 10500.0 + full * blocks * (block > fresh * pairs ? block : fresh * pairs);
-    if (rest > 0) clocks += blocks * (block > fresh * rest ? block : fresh * rest);
+    double clocks = 10500.0 + full * blocks * (all > fresh * pairs ? all : fresh * pairs);
+    const double last = 2 * rest > pairs && all > few ? all : few;
+    if (rest > 0) clocks += blocks * (last > fresh * rest ? last : fresh * rest);
     if (best.rows == 0 || clocks < best.clocks) best = {rows, 1, clocks};
-    // A tile's K cut in parts, where all clusters run at once; the sums' way through shared memory takes a part of the rows.
     for (int parts = 2; direct && parts <= 4 && blocks >= 4 * parts; parts *= 2) {
       if (tiles * parts > pairs || tiles > wide_clusters(parts)) break;
-      const double own = (blocks + parts - 1) / parts, split = block > fresh * tiles * parts ? block : fresh * tiles * parts;
-      const double time = 10500.0 + 2500.0 + 6.0 * rows + own * split;
+      const int own = (blocks + parts - 1) / parts;
+      const double block = 2 * tiles * parts > pairs && all > few ? all : few, hbm = fresh * tiles * parts;
+      const double fixed = parts == 2 ? 11500.0 + 0.13 * rows * rows : 13000.0 + 0.18 * rows * rows;
+      const double time = fixed + own * (block > hbm ? block : hbm);
       if (time < best.clocks) best = {rows, parts, time};
     }
   }
@@ -78,20 +79,26 @@ struct FewPlan {
   double clocks;
 };
 FewPlan plan_few(const Product& p) {
-  const int rows = p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128, blocks = (p.k + 63) / 64, sms = sm_count();
-  const long long row_tiles = (p.m + rows - 1) / rows, tiles = few_tiles(p) * row_tiles;
-  const int split = few_split(tiles, blocks, 2), own = (blocks + split - 1) / split;
-  const double alone = rows == 16 ? 367.0 : rows == 32 ? 378.0 : rows == 64 ? 487.0 : 627.0;
-  const double both = 2.0 * (16384.0 + 128.0 * rows) / 62.0;  // two CTAs on an SM
-  const double fixed = 8500.0 + 15.0 * rows + (split >= 4 ? 1500.0 : split == 2 ? 800.0 : 0.0);
-  const double fresh = 16384.0 / row_tiles / kHbmBytes;
-  const long long ctas = tiles * split, full = ctas / (2 * sms), rest = ctas % (2 * sms);
-  double clocks = fixed + full * own * (both > fresh * 2 * sms ? both : fresh * 2 * sms);
-  if (rest > 0) {
-    const double last = rest <= sms ? alone : both;
-    clocks += own * (last > fresh * rest ? last : fresh * rest);
+  const int blocks = (p.k + 63) / 64, sms = sm_count();
+  FewPlan best = {0, 1, 0.0};
+  for (int rows = 16; rows <= 128; rows *= 2) {
+    const long long row_tiles = (p.m + rows - 1) / rows, tiles = few_tiles(p) * row_tiles;
+    if (row_tiles > 8 && rows < 128) continue;
+    if (rows > 16 && rows / 2 >= p.m) break;
+    const int split = few_split(tiles, blocks, 2), own = (blocks + split - 1) / split;
+    const double alone = rows == 16 ? 367.0 : rows == 32 ? 378.0 : rows == 64 ? 487.0 : 627.0;
+    const double both = 2.0 * (16384.0 + 128.0 * rows) / 62.0;  // two CTAs on an SM
+    const double fixed = rows == 16 ? 9500.0 : rows == 32 ? 11000.0 : rows == 64 ? 13500.0 : 16500.0;
+    const double fresh = 16384.0 / row_tiles / kHbmBytes;
+    const long long ctas = tiles * split, full = ctas / (2 * sms), rest = ctas % (2 * sms);
+    double clocks = fixed + full * own * (both > fresh * 2 * sms ? both : fresh * 2 * sms);
+    if (rest > 0) {
+      const double last = rest <= sms ? alone : both;
+      clocks += own * (last > fresh * rest ? last : fresh * rest);
+    }
+    if (best.rows == 0 || clocks < best.clocks) best = {rows, split, clocks};
   }
-  return {rows, split, clocks};
+  return best;
 }
 
 int launch_dense_wide(const Product& p, const WidePlan& plan, cudaStream_t stream) {
