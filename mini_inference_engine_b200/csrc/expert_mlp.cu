@@ -2,10 +2,18 @@
 //
 //   y[t] = res[t] + sum_j w[t, j] D_e (act(G_e x[t]) * (U_e x[t])),   e = ids[t, j]
 //
+// Up to 32 tokens two launches (product_narrow.cuh).  More of them:
+//
 //   expert_plan_kernel     sorts the (token, choice) pairs by expert and cuts every expert's rows into tiles
-//   gate and up product    rows of x gathered by pair, activation, gate and the pair's weight in the epilogue
-//   down product           one row of sums per pair, in the pairs' own order
+//   gate and up product    rows of x gathered by pair; activation, gate and the pair's weight in the epilogue; one rounding to
+//                          bf16, which the tensor cores take
+//   down product           a row of sums per pair, as fp16 with an exponent per 32 entries: as bf16 the sum over the pairs would
+//                          lose as much again as by the hidden rows' rounding, as fp32 its rows would be twice the bytes
 //   expert_combine_kernel  adds a token's rows and the residual
+//
+// 8192 tokens of 2048 x 768, 8 of 128 experts (us, one after the other without a launch chain): 14, 304, 196, 86.  The products
+// are bound as product_wide.cuh says (the down product also by its 268 MB of rows, which HBM takes beside the weights), the sum
+// by HBM.  Together 620 us in a burst, 715 to 750 back to back under the power cap; the products' floor is 380.
 //
 // A pair's order among its expert's rows is whatever the counters gave; every row of a product is computed by itself, so
 // the results do not depend on it.  Ids outside [0, experts) take no part: -1 says "no expert", others also set a status bit.

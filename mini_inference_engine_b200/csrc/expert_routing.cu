@@ -7,7 +7,8 @@
 // 8, 16 or 32 lanes take a token (32 / lanes of them a warp), runs of V experts a lane, so that the lowest lane that has the
 // largest value has the lowest index.  Every lane sorts its run once; a choice is then one maximum over the token's lanes'
 // heads, and the lane that has it moves on.  Little data and many dependent steps: bound by instruction issue for many tokens
-// and by latency for few.
+// and by latency for few.  One token of 128 3.3 us, 30011 of 64 8.0, 4096 of 256 by groups and bias 15.6 (its bytes 0.7; a lane
+// that scanned its run for every choice took 18.1 of the second, 39.5 of the third with whole rows decided again in 64 bits).
 //
 // The choice is that of 64 bits.  Without a bias, and with groups judged by their best expert, the order of the scores is the
 // order of the logits, which are compared as they are.  Otherwise c is computed in 32 bits with an error below 2^-19 (1 + |c|)

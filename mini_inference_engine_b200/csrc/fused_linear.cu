@@ -1,4 +1,5 @@
-// Projections with bias, activation or gate, and residual in their epilogue.
+// Projections with bias, activation or gate, and residual in their epilogue: by streams of the weights for few rows
+// (product_narrow.cuh), on CTA pairs for many (product_wide.cuh), by single loads where a row is not 16-byte aligned.
 #include "product_narrow.cuh"
 #include "product_wide.cuh"
 #include "products.cuh"

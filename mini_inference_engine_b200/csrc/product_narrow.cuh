@@ -12,6 +12,11 @@
 //           few_parts); where an expert ends its part is taken out of tensor memory and added, with its weights, to the rows
 //           that are sent there and to no others (an expert's infinities stay with its rows).
 //
+// Measured: 1 row of 12288 x 2048 gated 12.0 us, 24 rows of 2560 x 9728 12.8 (their bytes 7.7 each): about 2 us from the start to
+// the first weights, 1.5 to 3 from the last ones to the end, growing with the rows, and what two CTAs an SM with 100 KB of ring
+// each get from HBM between.  A routed layer of 128 experts (2048 x 768, 8 a token) 22.4 us for 1 token (11.6), 79 for 8 (65),
+// 146 for 32 (121).
+//
 // Which experts are in use every CTA finds out by itself from the ids, a few hundred at most.  kUp lets the kernel after it
 // start behind its own wait for the kernels before: kDown may read the ids, and ask for its first weights, while kUp runs.
 #pragma once
@@ -31,7 +36,7 @@ constexpr int kFewPairs = kFewRoutedRows * MIE_MAX_TOP_K;
 template <int BN, Few kKind>
 struct FewSmem {
   static constexpr int kStageBytes = 128 * 128 + BN * 128;
-  static constexpr int kCtasPerSm = 2;
+  static constexpr int kCtasPerSm = 2;  // one CTA's ring alone does not cover HBM's latency
   static constexpr int kParkBytes = BN * 128 * 4;  // kUp: its own, the others' is the idle ring
   static constexpr int kRouting = kKind == Few::kDense ? 0 : kFewPairs * 6 + MIE_MAX_EXPERTS * 2 + 256;
   static constexpr int kExtra = kRouting + (kKind == Few::kUp ? kParkBytes : 0);

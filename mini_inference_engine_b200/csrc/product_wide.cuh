@@ -3,12 +3,26 @@
 // A pair (`cta_group::2`) multiplies 256 weight rows, 128 of each CTA, with up to 256 rows of x, half of which each CTA
 // stages: the weight rows are the M of the tensor-memory accumulator, the rows of x its N, so that a tile of few rows (the
 // end of an expert's) takes a multiple of 16 columns' time and not 256.  Two accumulators: the epilogue of a tile runs under
-// the products of the next.  One warp requests operands (128-byte-swizzled TMA tiles, rows of x by `tile::gather4` where
-// they are scattered), one issues the MMAs of the pair, eight finish.
+// the products of the next.  One warp requests operands by 128-byte-swizzled TMA tiles, eight more those rows of x that are
+// scattered (`tile::gather4`), one issues the MMAs of the pair, eight finish.
 //
-// Gated weights are staged as runs of 8 gates and 8 ups: the accumulator fragment of a thread (16 x 256b: channels l / 4 and
-// l / 4 + 8 of lane l) then holds a gate and its up.  Finished values go through shared memory, transposed by `stmatrix`, to
-// whole 128- or 256-byte runs of y's rows.
+// What bounds it.  A block of 64 columns is 512 clocks of products at 256 rows, and 64 KB of operands a pair, 64 bytes a clock
+// and SM: the products and L2 are about even, and under the power cap both.  8192 x 12288 x 4096 takes 536 us (1.54 PFLOP/s) in
+// a burst and 620 to 640 back to back (1.3, at the clocks that 1000 W allow), the gate_up product of 65536 routed rows 304 us
+// (1.36).  Smaller tiles load more per product: they are taken where fewer rounds or a fuller GPU are worth it (the caller's
+// plan).  What else cost time on the way: gathers issued by one warp (75 to 90 clocks a request: 902 us with one warp, 455
+// with four, 337 with eight and the rows' numbers in uniform registers, 308 apart from the weights' loads); handing an
+// accumulator back with a release, which waits for the rows stored before (264 -> 207 us of down product); activations one by
+// one (190 clocks each); finished values through shared memory, whose bandwidth the MMAs' operands take.
+//
+// So finished values go to y straight from the accumulator where they can (kDirect): the weight rows of a run of 32 are staged
+// in the order 4 s + j -> 8 j + s, and a thread's four accumulators of a row of x (fragments 16 x 256b: lanes l / 4 and l / 4 + 8
+// of either half) are neighbours in y.  Gated weights are staged as runs of 8 gates and 8 ups, a thread has a gate and its up,
+// and the values go through shared memory, transposed by `stmatrix`, to whole runs of y's rows, as they do where y's rows are
+// not whole runs of four.
+//
+// Where a product has fewer tiles than pairs, the K of a tile may be cut over the pairs of a cluster (kDense, kDirect), which
+// park their sums in the idle ring and each finish a part of the rows.
 #pragma once
 
 #include "products.cuh"
@@ -20,7 +34,7 @@ namespace {
 enum class Rows {
   kDense,  // y rows as x rows, bias, activation or gate, residual
   kUp,     // routed, gated: x gathered by pair, hidden rows in sorted order with the pair's weight
-  kDown    // routed: sorted hidden rows, y rows by pair as scaled fp16
+  kDown    // routed: sorted hidden rows, y rows in the same order as scaled fp16
 };
 
 // Finished values go to y straight from the accumulator's fragments (kDirect), or through shared memory.
@@ -342,9 +356,7 @@ __global__ void __launch_bounds__(wide_threads<kRows>(), 1)
       }
     }
   } else if constexpr (kDirect) {
-    // The weight rows of a run of 32 are staged in the order 4 s + j -> 8 j + s, so that a thread's four accumulators of a
-    // row of x are neighbours in y: 8 bytes a thread, 64 a row of y and warp, no shared memory (whose bandwidth the MMAs'
-    // operands take: the staged form's loads took 200 clocks each).
+    // 8 bytes a thread, 64 a row of y and warp.
     const int group = warp >> 2, quad = warp & 3, sub = lane >> 2, pick = lane & 3;
     int round = 0;
     bool ok = true;  // once a wait ran out nothing is stored
