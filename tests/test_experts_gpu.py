@@ -314,6 +314,81 @@ def test_large_and_small_values(magnitude, device):
         assert_within(out, *exact_expert_mlp(x, ids, weights, gate_up, down, "silu", None))
 
 
+@pytest.mark.parametrize("tokens", [1, 6, 20, 32, 33, 400])
+def test_the_same_call_gives_the_same_bits(tokens, device):
+    """Pairs are placed, and parts of sums arrive, in any order; the results do not depend on it."""
+
+    torch.manual_seed(11)
+    gate_up, down = pool(40, 512, 256, device)
+    x, r = torch.randn(tokens, 512, device=device).bfloat16(), torch.randn(tokens, 512, device=device).bfloat16()
+    ids = torch.argsort(torch.rand(tokens, 40, device=device), dim=1)[:, :6].to(torch.int32)
+    weights = torch.rand(tokens, 6, device=device)
+    status = torch.zeros(1, dtype=torch.int32, device=device)
+    first = expert_mlp(x, ids, weights, gate_up, down, residual=r, status=status)
+    for _ in range(20):
+        assert torch.equal(expert_mlp(x, ids, weights, gate_up, down, residual=r, status=status), first)
+
+
+@pytest.mark.parametrize("tokens", [1, 8, 32, 40, 200])
+def test_an_expert_that_is_no_number_stays_with_its_tokens(tokens, device):
+    torch.manual_seed(12)
+    gate_up, down = pool(12, 256, 128, device)
+    x = torch.randn(tokens, 256, device=device).bfloat16()
+    ids = torch.argsort(torch.rand(tokens, 12, device=device), dim=1)[:, :3].to(torch.int32)
+    ids[0] = torch.tensor([5, 1, 2], device=device)
+    weights = torch.rand(tokens, 3, device=device)
+    status = torch.zeros(1, dtype=torch.int32, device=device)
+    clean = expert_mlp(x, ids, weights, gate_up, down, status=status)
+    for broken in (float("nan"), float("inf")):
+        gate, out = gate_up.clone(), down.clone()
+        gate[5, 3, 7] = broken
+        out[5, 9, 11] = broken
+        touched = (ids == 5).any(dim=1)
+        for g, d in ((gate, down), (gate_up, out)):
+            got = expert_mlp(x, ids, weights, g, d, status=status)
+            assert torch.equal(got[~touched], clean[~touched])
+            assert not bool(torch.isfinite(got[0]).all())
+        # Of the down weight only its own channel (the others' rows may be rounded by another exponent).
+        others = torch.arange(256, device=device) != 9
+        exact, bound = exact_expert_mlp(x, ids, weights, gate_up, down, "silu", None)
+        assert_within(got[:, others], exact[:, others], bound[:, others])
+
+
+def test_all_experts_in_use_of_a_large_pool(device):
+    """1024 experts, 32 of them a token: the most a token may name."""
+
+    for tokens in (1, 32, 70):
+        torch.manual_seed(tokens)
+        gate_up, down = pool(1024, 64, 32, device)
+        x = torch.randn(tokens, 64, device=device).bfloat16()
+        ids = torch.argsort(torch.rand(tokens, 1024, device=device), dim=1)[:, :32].to(torch.int32)
+        weights = torch.rand(tokens, 32, device=device)
+        status = torch.zeros(1, dtype=torch.int32, device=device)
+        out = expert_mlp(x, ids, weights, gate_up, down, status=status)
+        assert_within(out, *exact_expert_mlp(x, ids, weights, gate_up, down, "silu", None))
+        assert int(status.item()) == 0
+
+
+def test_weights_routed_by_the_call_before(device):
+    """Ids and weights that a queued kernel writes, and a pool that the one before it wrote."""
+
+    torch.manual_seed(13)
+    status = torch.zeros(1, dtype=torch.int32, device=device)
+    for tokens in (1, 7, 20, 100):
+        gate_up, down = pool(16, 256, 128, device)
+        x = torch.randn(tokens, 256, device=device).bfloat16()
+        router = torch.randn(16, 256, device=device).bfloat16()
+        eye = torch.eye(128, dtype=torch.bfloat16, device=device)
+        for _ in range(10):
+            copy = torch.empty_like(down)
+            for e in range(16):
+                copy[e] = fused_linear(down[e], eye, status=status)
+            ids, weights = route_experts(fused_linear(x, router, status=status), 4, status=status)
+            out = expert_mlp(x, ids, weights, gate_up, copy, status=status)
+            expected = expert_mlp(x, ids.clone(), weights.clone(), gate_up, down, status=status)
+            assert torch.equal(out, expected)
+
+
 def test_feed_forward_refuses(device):
     x, gate_up, down = torch.zeros(2, 16, device=device).bfloat16(), *pool(4, 16, 8, device)
     ids, weights = torch.zeros(2, 2, dtype=torch.int32, device=device), torch.zeros(2, 2, device=device)
