@@ -11,9 +11,9 @@
 //                          lose as much again as by the hidden rows' rounding, as fp32 its rows would be twice the bytes
 //   expert_combine_kernel  adds a token's rows and the residual
 //
-// 8192 tokens of 2048 x 768, 8 of 128 experts (us, one after the other without a launch chain): 14, 304, 196, 86.  The products
-// are bound as product_wide.cuh says (the down product also by its 268 MB of rows, which HBM takes beside the weights), the sum
-// by HBM.  Together 620 us in a burst, 715 to 750 back to back under the power cap; the products' floor is 380.
+// 8192 tokens of 2048 x 768, 8 of 128 experts (us, one after the other without a launch chain): 14, 304 to 328, 196 to 207, 86.  The products
+// are bound as product_wide.cuh says (the down product also by its 268 MB of rows, which HBM takes beside the weights); the
+// sum moves its 340 MB at 0.6 of the copy rate.  Together 620 us in a burst, 715 to 780 back to back; the products' floor is 380.
 //
 // A pair's order among its expert's rows is whatever the counters gave; every row of a product is computed by itself, so
 // the results do not depend on it.  Ids outside [0, experts) take no part: -1 says "no expert", others also set a status bit.

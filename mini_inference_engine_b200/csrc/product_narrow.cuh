@@ -14,8 +14,8 @@
 //
 // Measured: 1 row of 12288 x 2048 gated 12.0 us, 24 rows of 2560 x 9728 12.8 (their bytes 7.7 each): about 2 us from the start to
 // the first weights, 1.5 to 3 from the last ones to the end, growing with the rows, and what two CTAs an SM with 100 KB of ring
-// each get from HBM between.  A routed layer of 128 experts (2048 x 768, 8 a token) 22.4 us for 1 token (11.6), 79 for 8 (65),
-// 146 for 32 (121).
+// each get from HBM between.  A routed layer of 128 experts (2048 x 768, 8 a token) 22.4 us for 1 token (11.6), 79 for 8 (65 if
+// their experts are spread evenly, fewer are read where some are favoured), 146 for 32 (121 by the same count).
 //
 // Which experts are in use every CTA finds out by itself from the ids, a few hundred at most.  kUp lets the kernel after it
 // start behind its own wait for the kernels before: kDown may read the ids, and ask for its first weights, while kUp runs.
