@@ -317,8 +317,11 @@ __device__ __forceinline__ float warp_max(float v) {
 int make_tensor_map(CUtensorMap* out, CUtensorMapDataType dtype, int rank, void* base, const uint64_t* dims,
                     const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swizzle);
 
-// The same for bf16 operands, 64 elements (128 bytes, swizzled) wide, from a cache by all of its arguments.
-int cached_operand_map(CUtensorMap* out, int rank, const void* base, const uint64_t* dims, const uint64_t* strides_bytes,
-                       const uint32_t* box);
+// The same for bf16 operands, 64 elements (128 bytes, swizzled) wide.
+inline int operand_map_bf16(CUtensorMap* out, int rank, const void* base, const uint64_t* dims, const uint64_t* strides_bytes,
+                            const uint32_t* box) {
+  return make_tensor_map(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides_bytes, box,
+                         CU_TENSOR_MAP_SWIZZLE_128B);
+}
 
 }  // namespace mie

@@ -388,7 +388,7 @@ int launch_routed_few(const Product& up, const Product& out, FewParams q, cudaSt
   const uint64_t dims[3] = {(uint64_t)out.k, (uint64_t)BN, (uint64_t)most};
   const uint64_t strides[2] = {(uint64_t)out.ldx * 2, (uint64_t)out.ldx * 2 * BN};
   const uint32_t box[3] = {64, (uint32_t)BN, 1};
-  if (int rc = cached_operand_map(&map_x, 3, out.x, dims, strides, box)) return rc;
+  if (int rc = operand_map_bf16(&map_x, 3, out.x, dims, strides, box)) return rc;
   const int cluster = few_split(q.weight_tiles, (int)most * ((out.k + 63) / 64), 2), parts = few_parts(out.n, pairs, cluster);
   if (parts == 0) q.parts = nullptr;
   return launch_few<BN, Few::kDown, false>(map_w, map_x, q, q.weight_tiles, parts > 0 ? parts : cluster, 1, stream);

@@ -513,7 +513,7 @@ inline int few_weight_map(CUtensorMap* out, const Product& p, int experts, int b
   const uint64_t dims[3] = {(uint64_t)p.k, (uint64_t)p.n * (p.gated ? 2 : 1), (uint64_t)experts};
   const uint64_t strides[2] = {row, experts > 1 ? (uint64_t)p.w_expert * 2 : row};
   const uint32_t box[3] = {64, (uint32_t)box_rows, 1};
-  return cached_operand_map(out, 3, p.w, dims, strides, box);
+  return operand_map_bf16(out, 3, p.w, dims, strides, box);
 }
 
 template <int BN, Few kKind, bool kGated>

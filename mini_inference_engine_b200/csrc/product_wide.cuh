@@ -773,7 +773,7 @@ inline int weight_maps(WeightMaps* out, const Product& p, int experts, bool dire
     const uint64_t dims[3] = {k, (uint64_t)p.n, (uint64_t)experts};
     const uint64_t strides[2] = {row, expert};
     const uint32_t box[3] = {64, 128, 1};
-    return cached_operand_map(&out->all, 3, p.w, dims, strides, box);
+    return operand_map_bf16(&out->all, 3, p.w, dims, strides, box);
   }
   // Runs: [8 rows][gate, up] or [8 rows 4 apart][4 rows].
   const uint32_t inner = p.gated ? 2 : 4, runs = p.gated ? 8 : 4;
@@ -785,15 +785,15 @@ inline int weight_maps(WeightMaps* out, const Product& p, int experts, bool dire
   const uint64_t rest_rows = (uint64_t)(p.gated ? rest : rest / 4);
   const uint64_t rest_dims[5] = {k, rest > 0 ? rest_rows : 8, inner, 1, (uint64_t)experts};
   const __nv_bfloat16* rest_base = rest > 0 ? p.w + (long long)whole * run * p.ldw : p.w;
-  if (int rc = cached_operand_map(&out->all, 5, p.w, dims, strides, box)) return rc;
-  if (int rc = cached_operand_map(&out->run, 5, p.w, dims, strides, one)) return rc;
-  return cached_operand_map(&out->rest, 5, rest_base, rest_dims, strides, one);
+  if (int rc = operand_map_bf16(&out->all, 5, p.w, dims, strides, box)) return rc;
+  if (int rc = operand_map_bf16(&out->run, 5, p.w, dims, strides, one)) return rc;
+  return operand_map_bf16(&out->rest, 5, rest_base, rest_dims, strides, one);
 }
 inline int row_map(CUtensorMap* out, const Product& p, long long rows, int box_rows) {
   const uint64_t dims[2] = {(uint64_t)p.k, (uint64_t)rows};
   const uint64_t strides[1] = {(uint64_t)p.ldx * 2};
   const uint32_t box[2] = {64, (uint32_t)box_rows};
-  return cached_operand_map(out, 2, p.x, dims, strides, box);
+  return operand_map_bf16(out, 2, p.x, dims, strides, box);
 }
 // What the pair kernel's loads ask of the operands.
 inline bool wide_takes(const Product& p) {

@@ -2,13 +2,10 @@
 #include <stdarg.h>
 #include <stdio.h>
 #include <stdlib.h>
-#include <string.h>
 
 #include <atomic>
-#include <exception>
 #include <mutex>
 #include <set>
-#include <unordered_map>
 #include <utility>
 
 #include "common.cuh"
@@ -117,54 +114,6 @@ int make_tensor_map(CUtensorMap* out, CUtensorMapDataType dtype, int rank, void*
                   swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled failed with CUresult %d (rank %d, base %p)", (int)r, rank, base);
-    return MIE_ERR_CUDA;
-  }
-  return MIE_OK;
-}
-
-namespace {
-struct OperandMapKey {
-  uint64_t words[16];
-  bool operator==(const OperandMapKey& o) const { return memcmp(words, o.words, sizeof(words)) == 0; }
-};
-struct OperandMapHash {
-  size_t operator()(const OperandMapKey& k) const {
-    size_t h = 0;
-    for (uint64_t w : k.words) h = h * 1000003u ^ (size_t)w;
-    return h;
-  }
-};
-}  // namespace
-
-int cached_operand_map(CUtensorMap* out, int rank, const void* base, const uint64_t* dims, const uint64_t* strides_bytes,
-                       const uint32_t* box) {
-  static std::mutex mu;
-  static std::unordered_map<OperandMapKey, CUtensorMap, OperandMapHash> cache;
-  OperandMapKey key = {};
-  key.words[0] = (uint64_t)reinterpret_cast<uintptr_t>(base);
-  for (int i = 0; i < rank; ++i) {
-    key.words[1 + i] = dims[i];
-    key.words[6 + i] = box[i];
-    if (i > 0) key.words[10 + i] = strides_bytes[i - 1];
-  }
-  key.words[15] = (uint64_t)rank;
-  try {
-    {
-      std::lock_guard<std::mutex> lock(mu);
-      auto it = cache.find(key);
-      if (it != cache.end()) {
-        *out = it->second;
-        return MIE_OK;
-      }
-    }
-    if (int rc = make_tensor_map(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides_bytes,
-                                 box, CU_TENSOR_MAP_SWIZZLE_128B))
-      return rc;
-    std::lock_guard<std::mutex> lock(mu);
-    if (cache.size() > 4096) cache.clear();
-    cache.emplace(key, *out);
-  } catch (const std::exception& e) {
-    set_error("%s while a tensor map was looked up", e.what());
     return MIE_ERR_CUDA;
   }
   return MIE_OK;
