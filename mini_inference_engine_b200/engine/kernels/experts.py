@@ -8,7 +8,7 @@ import functools
 import torch
 
 from ... import _lib
-from .linear import activation_code, check_rows
+from .linear import activation_code, check_rows, check_sizes, check_status
 
 MAX_EXPERTS = 1024  # MIE_MAX_EXPERTS
 MAX_TOP_K = 32      # MIE_MAX_TOP_K
@@ -34,6 +34,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scores: str = "softmax", 
     NaN."""
 
     del status  # every input is valid on the device
+    check_sizes(*logits.shape, top_k)
     if logits.ndim != 2 or logits.dtype not in _lib.DTYPE_CODES or not logits.is_cuda:
         raise ValueError("route_experts takes CUDA logits [tokens, experts] in bf16, fp16 or fp32")
     if scores not in SCORES:
@@ -75,6 +76,7 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate_u
     code, device = activation_code(activation), x.device
     (tokens, width), (experts, double_ff, _), top_k = x.shape, gate_up.shape, int(ids.shape[1])
     ff = double_ff // 2
+    check_sizes(tokens, width, experts, double_ff, top_k)
     ldx, _ = check_rows("x", x, (tokens, width), device)
     gate_up_row, gate_up_expert = check_rows("gate_up", gate_up, (experts, 2 * ff, width), device)
     down_row, down_expert = check_rows("down", down, (experts, width, ff), device)
@@ -86,6 +88,7 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate_u
         raise ValueError(f"weights must be dense fp32 {list(ids.shape)} on the device of x")
     if weights.requires_grad and torch.is_grad_enabled():
         raise ValueError("weights requires a gradient: this operator has none")
+    check_status(status, device)
     out = torch.empty((tokens, width), dtype=torch.bfloat16, device=device)
     if tokens == 0:
         return out

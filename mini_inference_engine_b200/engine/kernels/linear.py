@@ -96,6 +96,18 @@ def check_rows(name: str, tensor: torch.Tensor, shape: tuple[int, ...], device: 
     return leading[0] if leading else width, leading[1] if len(leading) > 1 else matrix
 
 
+def check_sizes(*sizes: int) -> None:
+    """The library takes sizes of 32 bits."""
+
+    if max(sizes) >= 1 << 31:
+        raise ValueError(f"sizes up to 2^31 - 1, not {max(sizes)}")
+
+
+def check_status(status: torch.Tensor, device: torch.device) -> None:
+    if status.dtype is not torch.int32 or status.device != device or status.numel() < 1:
+        raise ValueError(f"status must be an int32 word on {device}")
+
+
 def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
                  activation: str | None = None, gated: bool = False, residual: torch.Tensor | None = None,
                  status: torch.Tensor) -> torch.Tensor:
@@ -108,6 +120,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     code, device = activation_code(activation), x.device
     rows, k = x.shape
     n = weight.shape[0]
+    check_sizes(rows, n, k)
     ldx, _ = check_rows("x", x, (rows, k), device)
     ldw, _ = check_rows("weight", weight, (n, k), device)
     if bias is not None:
@@ -119,6 +132,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     if n < 1 or k < 1:
         raise ValueError("fused_linear needs at least one column and one weight row")
     ldr = 0 if residual is None else check_rows("residual", residual, (rows, n), device)[0]
+    check_status(status, device)
     out = torch.empty((rows, n), dtype=torch.bfloat16, device=device)
     if rows == 0:
         return out

@@ -28,6 +28,13 @@ def test_refusals_of_the_operators():
         expert_mlp(x, ids, weights, gate_up, down, activation="swish", status=status)
     with pytest.raises(ValueError, match="takes x"):
         expert_mlp(x, ids, weights, gate_up[0], down, status=status)
+    long = torch.zeros(1, 1).bfloat16().expand(1 << 31, 1)
+    with pytest.raises(ValueError, match="sizes up to"):
+        route_experts(long, 1)
+    with pytest.raises(ValueError, match="sizes up to"):
+        route_experts(torch.zeros(2, 8), (1 << 32) + 1)
+    with pytest.raises(ValueError, match="sizes up to"):
+        expert_mlp(long, ids, weights, gate_up, down, status=status)
     with pytest.raises(ValueError, match="must be bf16"):
         expert_mlp(x.float(), ids, weights, gate_up, down, status=status)
 

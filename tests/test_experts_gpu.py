@@ -461,3 +461,14 @@ def test_a_routed_layer(tokens, device):
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(beside, here))
     assert int(status.item()) == 0
+
+
+def test_a_status_that_the_device_cannot_write(device):
+    x, gate_up, down = torch.zeros(2, 16, device=device).bfloat16(), *pool(4, 16, 8, device)
+    ids, weights = torch.zeros(2, 2, dtype=torch.int32, device=device), torch.zeros(2, 2, device=device)
+    for status in (torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int64, device=device),
+                   torch.zeros(0, dtype=torch.int32, device=device)):
+        with pytest.raises(ValueError, match="int32 word"):
+            expert_mlp(x, ids, weights, gate_up, down, status=status)
+        with pytest.raises(ValueError, match="int32 word"):
+            fused_linear(x, x, status=status)

@@ -26,6 +26,7 @@ def rows(r, c, dtype=torch.bfloat16):
     (rows(2, 8), rows(4, 8), {"activation": "swish"}, "unknown activation"),
     (rows(2, 8, torch.float32), rows(4, 8), {}, "must be bf16"),
     (rows(2, 8).view(1, 2, 8), rows(4, 8), {}, "takes rows"),
+    (rows(1, 1).expand(1 << 32, 1), rows(4, 1), {}, "sizes up to"),
 ])
 def test_refusals_of_the_operator(x, w, options, message):
     with pytest.raises(ValueError, match=message):
