@@ -15,7 +15,9 @@
 // (approximate exponential and reciprocal 2^-22 each, the argument's rounding, a sum of up to 1024 terms, the bias' addition,
 // of a value in [0, 1] or of c).  Where two values that decide something are nearer than twice that and do not come from
 // equal logits and biases, the choice goes on to whatever is as near, and those candidates are ordered by c in 64 bits (all
-// experts, where there are more than 32).  Groups that are as near are decided again first.
+// experts, where there are more than 32).  Neighbours are compared down to the first one left out; where that one equals the
+// last one taken, the others are looked through for one as near (has_rival; 4096 equal rows of 256 12.7 -> 24.1 us, rows without
+// equals at the border within 1 %).  Groups that are as near are decided again first.
 #include "common.cuh"
 #include "glue.cuh"
 
@@ -205,6 +207,34 @@ __device__ __noinline__ void order_candidates(const RouteParams& p, const T* row
   __syncwarp();
   if (lane < count) ids[rank] = e;
   __syncwarp();
+}
+
+// Equal in every number of bits: equal logits and biases, or both masked.
+template <typename T>
+__device__ __forceinline__ bool same_choice(const RouteParams& p, const T* row, int a, int b) {
+  const float za = to_float<T>(row[a]), zb = to_float<T>(row[b]);
+  return (za == zb && (p.bias == nullptr || p.bias[a] == p.bias[b])) || (za == -INFINITY && zb == -INFINITY);
+}
+
+// Whether the groups `kept` have an expert that 32 bits do not tell from `last` though it is another choice, by a whole warp.
+// (These c and those that were compared are off by 2^-19 each: twice the distance.)
+template <typename T>
+__device__ __noinline__ bool has_rival(const RouteParams& p, const T* row, float top, float sum, uint32_t kept, int last) {
+  const int lane = threadIdx.x & 31, size = p.experts / p.groups;
+  auto choice = [&](int e) {
+    const float z = to_float<T>(row[e]);
+    if (z == -INFINITY) return z;
+    return (p.sigmoid ? 1.f / (1.f + expf(-z)) : expf(z - top) / sum) + (p.bias != nullptr ? p.bias[e] : 0.f);
+  };
+  const float border = choice(last), near = 2.f * kUncertain * (1.f + fabsf(border));
+  if (border == -INFINITY) return false;  // so is all that is left, in the order of the indices
+  bool found = false;
+#pragma unroll 1
+  for (int e = lane; e < p.experts; e += 32) {
+    if (!((kept >> (p.groups > 1 ? e / size : 0)) & 1u)) continue;
+    found |= !(fabsf(border - choice(e)) > near) && !same_choice<T>(p, row, last, e);
+  }
+  return __any_sync(kAll, found);
 }
 
 // Descending by (key, low).
@@ -438,7 +468,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
     } else {
       uint32_t last = 0;
       int last_e = 0, count = 0;
-      bool near_ties = false;
+      bool near_ties = false, equal_border = false;  // the last expert taken and the first one left out
       float least = INFINITY;  // candidates are not below it
       for (int j = 0; j <= p.top_k || (j < 32 && __any_sync(kAll, near_ties && count == j)); ++j) {
         uint32_t best;
@@ -449,9 +479,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
         if (j > 0 && j <= p.top_k) {
           const float a = key_value(last);
           if (!far_apart(a, value, fabsf(a))) {
-            const float za = to_float<T>(row[last_e]), zb = to_float<T>(row[e]);
-            near_ties |= !((za == zb && (p.bias == nullptr || p.bias[last_e] == p.bias[e])) ||
-                           (za == -INFINITY && zb == -INFINITY));
+            const bool same = same_choice<T>(p, row, last_e, e);
+            near_ties |= !same;
+            equal_border = same && j == p.top_k;
           }
         }
         if (j == p.top_k - 1) least = value - 2.f * kUncertain * (1.f + fabsf(value));
@@ -460,7 +490,18 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
         last_e = e;
       }
       // More candidates than are held, or values that are no numbers: all over again.
-      const bool all_again = near_ties && (count >= 32 || !(least == least));
+      bool all_again = near_ties && (count >= 32 || !(least == least));
+      __syncwarp();
+      // Behind equals at the border there may be others as near, which no comparison of neighbours has seen.
+      uint32_t ask = __ballot_sync(kAll, equal_border && !near_ties);
+      while (ask != 0) {
+        const int s = (__ffs(ask) - 1) / L, from = s * L;
+        ask &= ~((L == 32 ? kAll : (1u << (L & 31)) - 1u) << from);
+        const T* which = reinterpret_cast<const T*>(p.logits) + __shfl_sync(kAll, t, from) * p.ld;
+        const bool rival = has_rival<T>(p, which, __shfl_sync(kAll, top, from), __shfl_sync(kAll, sum, from),
+                                        __shfl_sync(kAll, kept, from), chosen_all[warp][s][p.top_k - 1]);
+        if (own == s && rival) near_ties = all_again = true;
+      }
       uint32_t again = __ballot_sync(kAll, near_ties);
       __syncwarp();
       while (again != 0) {

@@ -166,6 +166,44 @@ def test_scores_far_below_one(device):
         check_route(low, 6, scores="softmax", bias=bias, renormalize=False)
 
 
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts", [3, 30, 64, 100, 256, 400, 1000])
+def test_equals_at_the_border_of_the_choice(experts, scores, device):
+    """The last expert taken and the first one left out have equal logits and biases, and a third one, behind them in 32 bits or
+    by its index, is better in 64."""
+
+    torch.manual_seed(experts)
+    near = max(3, experts // 2)
+    for top_k in sorted({1, 2, min(8, near - 1), min(32, near - 1)}):
+        for base in (-3.0, 0.7, 2.0):
+            # Logits of two values that are a rounding or two apart, at random places, with the others clearly below.
+            step = (torch.rand(60, experts, device=device) < 0.1).float()
+            logits = base * (1.0 + step * 2.0 ** -22)
+            low = torch.argsort(torch.rand(60, experts, device=device), dim=1)[:, near:]
+            logits.scatter_(1, low, base - 4.0)
+            bias = torch.randint(0, 2, (experts,), device=device).float() * 2.0 ** -20
+            for b in (torch.zeros(experts, device=device), torch.full((experts,), 0.3, device=device), bias):
+                check_route(logits.contiguous(), top_k, scores=scores, bias=b)
+                # (Mixed biases give groups whose sums are equal but for the roundings of 64 bits.)
+                if experts % 4 == 0 and b is not bias:
+                    check_route(logits.contiguous(), min(top_k, experts // 2), scores=scores, bias=b, groups=4, top_groups=2,
+                                group_best=2)
+
+
+def test_equal_saturated_scores_at_the_border(device):
+    """Sigmoids that are all one in 32 bits and not in 64."""
+
+    for experts in (3, 70, 300):
+        zero = torch.zeros(experts, device=device)
+        logits = torch.full((3, experts), 18.0, device=device)
+        logits[0, -1] = 20.0
+        logits[1, experts // 2] = 19.0
+        logits[1, -1] = 19.5
+        for top_k in (1, 2, min(32, experts - 1)):
+            check_route(logits, top_k, scores="sigmoid", bias=zero)
+            check_route(logits.bfloat16(), top_k, scores="sigmoid", bias=zero + 0.5)
+
+
 def test_logits_that_are_no_numbers(device):
     torch.manual_seed(4)
     logits = torch.randn(6, 40, device=device)
