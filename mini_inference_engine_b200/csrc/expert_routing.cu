@@ -517,19 +517,19 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
       }
     }
     __syncwarp();
-    // Over the chosen's sum only their ratios count: softmax goes by the largest of the chosen (all may be far below the row's),
-    // and so does sigmoid where it is exp(z) but for a factor of 1 - 2^-86 and may underflow.
-    float total = p.sigmoid ? 1.f : sum, shift = top;
-    bool ratio = !p.sigmoid;
+    // Over the chosen's sum only their ratios count.  So exponentials are taken against the largest of the chosen, which may be
+    // far below the row's; a sigmoid is exp(z) / (1 + exp(z)), and of it the numerator as long as the largest is below 0.
+    float total = p.sigmoid ? 1.f : sum, shift = p.sigmoid ? 0.f : top;
     if (p.renormalize) {
       shift = -INFINITY;
       for (int j = l; j < p.top_k; j += L) shift = fmaxf(shift, to_float<T>(row[chosen[j]]));
       shift = token_max<L>(shift);
-      ratio |= shift < -60.f;
+      if (p.sigmoid) shift = fminf(shift, 0.f);
     }
     auto weight = [&](float v) {
       if (v == -INFINITY) return 0.f;
-      return ratio ? expf(v - shift) : 1.f / (1.f + expf(-v));
+      if (!p.sigmoid) return expf(v - shift);
+      return v > 0.f ? 1.f / (1.f + expf(-v)) : expf(v - shift) / (1.f + expf(v));
     };
     if (p.renormalize) {
       total = 0.f;

@@ -204,6 +204,21 @@ def test_equal_saturated_scores_at_the_border(device):
             check_route(logits.bfloat16(), top_k, scores="sigmoid", bias=zero + 0.5)
 
 
+def test_sigmoid_weights_of_any_ratio(device):
+    """Weights over the chosen's sum whose sigmoids lie far apart, the smaller ones below what 32 bits hold.
+
+    Arguments of the exponentials are differences up to 128, rounded once (2^-18); exponentials, sums and divisions add less
+    than 2^-20: below 2^-17."""
+
+    torch.manual_seed(20)
+    for largest in (-59.9, -59.0, -40.0, -25.0, -10.0, 3.0):
+        logits = largest - 80.0 * torch.rand(50, 24, device=device)
+        logits[:, 5] = largest
+        for top_k in (2, 10, 24):
+            check_route(logits, top_k, scores="sigmoid")
+            check_route(logits, top_k, scores="sigmoid", bias=0.1 * torch.randn(24, device=device))
+
+
 def test_logits_that_are_no_numbers(device):
     torch.manual_seed(4)
     logits = torch.randn(6, 40, device=device)
