@@ -12,12 +12,27 @@ from .linear import activation_code, check_rows, check_sizes, check_status
 
 MAX_EXPERTS = 1024  # MIE_MAX_EXPERTS
 MAX_TOP_K = 32      # MIE_MAX_TOP_K
+MAX_GROUPS = 32
 SCORES = {"softmax": 0, "sigmoid": 1}  # MIE_SCORES_*
 
 
 @functools.lru_cache(maxsize=4096)
 def _scratch_bytes(tokens: int, top_k: int, experts: int, width: int, ff: int) -> int:
     return int(_lib.load().mie_expert_scratch_bytes(tokens, top_k, experts, width, ff))
+
+
+def _check_choice(experts: int, top_k: int, groups: int, top_groups: int, group_best: int) -> None:
+    """What the library refuses too, ahead of the results' allocation and of calls without tokens."""
+
+    if not 1 <= experts <= MAX_EXPERTS:
+        raise ValueError(f"routing takes up to {MAX_EXPERTS} experts, not {experts}")
+    if not 1 <= groups <= MAX_GROUPS or experts % groups or not 1 <= top_groups <= groups:
+        raise ValueError(f"{experts} experts cannot be chosen from {top_groups} of {groups} groups")
+    size = experts // groups
+    if not 1 <= group_best <= min(2, size):
+        raise ValueError("groups are judged by their best one or two")
+    if not 1 <= top_k <= min(MAX_TOP_K, top_groups * size):
+        raise ValueError(f"cannot choose {top_k} experts from {top_groups} groups of {size}")
 
 
 def route_experts(logits: torch.Tensor, top_k: int, *, scores: str = "softmax", bias: torch.Tensor | None = None,
@@ -34,12 +49,15 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scores: str = "softmax", 
     NaN."""
 
     del status  # every input is valid on the device
-    check_sizes(*logits.shape, top_k)
-    if logits.ndim != 2 or logits.dtype not in _lib.DTYPE_CODES or not logits.is_cuda:
+    check_sizes(*logits.shape, top_k, groups, top_groups, group_best)
+    if logits.ndim != 2 or logits.dtype not in _lib.DTYPE_CODES:
         raise ValueError("route_experts takes CUDA logits [tokens, experts] in bf16, fp16 or fp32")
     if scores not in SCORES:
         raise ValueError(f"unknown scores {scores!r}: one of {', '.join(SCORES)}")
-    tokens, experts = logits.shape
+    (tokens, experts), top_k = logits.shape, int(top_k)
+    _check_choice(experts, top_k, groups, top_groups, group_best)
+    if not logits.is_cuda:
+        raise ValueError("route_experts takes CUDA logits [tokens, experts] in bf16, fp16 or fp32")
     if experts > 1 and logits.stride(1) != 1 or tokens > 1 and logits.stride(0) < experts:
         raise ValueError(f"logits need dense rows that do not overlap, not strides {list(logits.stride())}")
     if bias is not None and (bias.dtype is not torch.float32 or tuple(bias.shape) != (experts,) or
@@ -47,9 +65,9 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scores: str = "softmax", 
         raise ValueError(f"bias must be dense fp32 [{experts}] on the logits' device")
     if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
         raise ValueError("route_experts has no gradient")
-    device, top_k = logits.device, int(top_k)
-    ids = torch.empty((tokens, max(top_k, 0)), dtype=torch.int32, device=device)
-    weights = torch.empty((tokens, max(top_k, 0)), dtype=torch.float32, device=device)
+    device = logits.device
+    ids = torch.empty((tokens, top_k), dtype=torch.int32, device=device)
+    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=device)
     if tokens == 0:
         return ids, weights
     with _lib.on_device(device):

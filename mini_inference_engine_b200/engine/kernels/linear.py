@@ -99,8 +99,8 @@ def check_rows(name: str, tensor: torch.Tensor, shape: tuple[int, ...], device: 
 def check_sizes(*sizes: int) -> None:
     """The library takes sizes of 32 bits."""
 
-    if max(sizes) >= 1 << 31:
-        raise ValueError(f"sizes up to 2^31 - 1, not {max(sizes)}")
+    if max(sizes) >= 1 << 31 or min(sizes) < -1 << 31:
+        raise ValueError(f"sizes up to 2^31 - 1, not {max(sizes, key=abs)}")
 
 
 def check_status(status: torch.Tensor, device: torch.device) -> None:

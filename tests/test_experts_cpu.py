@@ -77,3 +77,29 @@ def test_refusals_of_the_feed_forward(lib):
         assert experts_call(lib, **wrong) == -1, wrong
     assert lib.mie_expert_scratch_bytes(8, 2, 4, 16, 8) > 0
     assert lib.mie_expert_scratch_bytes(-1, 2, 4, 16, 8) == 0
+
+
+def test_refusals_of_choices():
+    """Before anything is allocated, and without tokens as well."""
+
+    far = 1 << 32
+    for tokens in (0, 2):
+        logits = torch.zeros(tokens, 16)
+        for options in ({"groups": far + 1}, {"top_groups": far + 1}, {"group_best": far + 1}, {"groups": 1 - far},
+                        {"groups": 4, "top_groups": 2 - far}):
+            with pytest.raises(ValueError, match="sizes"):
+                route_experts(logits, 2, **options)
+        for top_k, options in ((0, {}), (-1, {}), (17, {}), (5, {"groups": 4}), (1 << 30, {}), (33, {"logits": 64})):
+            z = torch.zeros(tokens, options.pop("logits", 16))
+            with pytest.raises(ValueError, match="cannot choose"):
+                route_experts(z, top_k, **options)
+        for options in ({"groups": 0}, {"groups": 3}, {"groups": 4, "top_groups": 5}, {"groups": 4, "top_groups": 0}):
+            with pytest.raises(ValueError, match="groups"):
+                route_experts(logits, 2, **options)
+        for options in ({"group_best": 0}, {"group_best": 3}, {"groups": 16, "top_groups": 4, "group_best": 2}):
+            with pytest.raises(ValueError, match="best"):
+                route_experts(logits, 2, **options)
+        with pytest.raises(ValueError, match="up to 1024 experts"):
+            route_experts(torch.zeros(tokens, 1025), 2)
+    with pytest.raises(ValueError, match="experts"):
+        route_experts(torch.zeros(2, 0), 1)
