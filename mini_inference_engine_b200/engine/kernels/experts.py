@@ -13,6 +13,7 @@ from .linear import activation_code, check_rows, check_sizes, check_status
 MAX_EXPERTS = 1024  # MIE_MAX_EXPERTS
 MAX_TOP_K = 32      # MIE_MAX_TOP_K
 MAX_GROUPS = 32
+MAX_PAIRS = 1 << 30  # of tokens and their experts
 SCORES = {"softmax": 0, "sigmoid": 1}  # MIE_SCORES_*
 
 
@@ -95,6 +96,11 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate_u
     (tokens, width), (experts, double_ff, _), top_k = x.shape, gate_up.shape, int(ids.shape[1])
     ff = double_ff // 2
     check_sizes(tokens, width, experts, double_ff, top_k)
+    if not (1 <= experts <= MAX_EXPERTS and 1 <= top_k <= MAX_TOP_K and width >= 1 and ff >= 1):
+        raise ValueError(f"expert_mlp takes up to {MAX_EXPERTS} experts, {MAX_TOP_K} of them a token, and rows of one entry or "
+                         f"more, not {top_k} of {experts} experts of {width} x {ff}")
+    if tokens * top_k >= MAX_PAIRS:
+        raise ValueError(f"too many (token, expert) pairs: {tokens} x {top_k}")
     ldx, _ = check_rows("x", x, (tokens, width), device)
     gate_up_row, gate_up_expert = check_rows("gate_up", gate_up, (experts, 2 * ff, width), device)
     down_row, down_expert = check_rows("down", down, (experts, width, ff), device)

@@ -103,3 +103,21 @@ def test_refusals_of_choices():
             route_experts(torch.zeros(tokens, 1025), 2)
     with pytest.raises(ValueError, match="experts"):
         route_experts(torch.zeros(2, 0), 1)
+
+
+def test_refusals_of_pools():
+    """Pools and choices that no call takes, with and without tokens, before scratch is asked for."""
+
+    status = torch.zeros(1, dtype=torch.int32)
+    for tokens in (0, 2):
+        for top_k, experts, width, ff in ((0, 4, 16, 8), (33, 64, 16, 8), (2, 0, 16, 8), (2, 1025, 16, 8), (2, 4, 0, 8),
+                                          (2, 4, 16, 0)):
+            given = (torch.zeros(tokens, width).bfloat16(), torch.zeros(tokens, top_k, dtype=torch.int32),
+                     torch.zeros(tokens, top_k), torch.zeros(experts, 2 * ff, width).bfloat16(),
+                     torch.zeros(experts, width, ff).bfloat16())
+            with pytest.raises(ValueError, match="expert_mlp takes"):
+                expert_mlp(*given, status=status)
+    ids, weights = torch.zeros(1, 1, dtype=torch.int32).expand(1 << 26, 16), torch.zeros(1, 1).expand(1 << 26, 16)
+    with pytest.raises(ValueError, match="pairs"):
+        expert_mlp(torch.zeros(1, 16).bfloat16().expand(1 << 26, 16), ids, weights, torch.zeros(4, 16, 16).bfloat16(),
+                   torch.zeros(4, 16, 8).bfloat16(), status=status)
