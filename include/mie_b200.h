@@ -489,6 +489,9 @@ int mie_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const voi
 #define MIE_ACT_GELU 2
 #define MIE_ACT_RELU 3
 
+/* Most rows, entries of a row, or columns of the products below: tiles are counted in 32 bits, past the last one as well. */
+#define MIE_MAX_PRODUCT 2147479552 /* 2^31 - 4096 */
+
 /*
  * Projection of bf16 rows with its epilogue: y[m, n] = act(x[m, k] w[n, k]^T + bias[n]) + residual[m, n]; gated: w and
  * bias have 2 n rows, gates first, and y = act(x w_g^T + bias_g) * (x w_u^T + bias_u) + residual.  fp32 sums and epilogue,

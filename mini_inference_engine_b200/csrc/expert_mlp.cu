@@ -408,7 +408,7 @@ int launch_any(const Product& p, long long tiles, cudaStream_t stream) {
 using namespace mie;
 
 extern "C" int64_t mie_expert_scratch_bytes(int32_t tokens, int32_t top_k, int32_t experts, int32_t width, int32_t ff) {
-  if (tokens < 0 || top_k < 1 || experts < 1 || width < 1 || ff < 1) return 0;
+  if (tokens < 0 || top_k < 1 || experts < 1 || width < 1 || ff < 1 || width > MIE_MAX_PRODUCT || ff > 1 << 30) return 0;
   return Scratch(tokens, top_k, experts, width, ff).total;
 }
 
@@ -419,8 +419,8 @@ extern "C" int mie_expert_mlp(const void* x, int64_t ldx, mie_index_t ids, const
                               int32_t activation, void* scratch, int64_t scratch_bytes, int32_t* status, void* stream_) {
   cudaStream_t stream = (cudaStream_t)stream_;
   MIE_CHECK_ARG(x && ids.ptr && weights && gate_up && down && y && scratch, "null pointer");
-  MIE_CHECK_ARG(tokens >= 0 && width >= 1 && ff >= 1 && experts >= 1 && experts <= MIE_MAX_EXPERTS && top_k >= 1 &&
-                    top_k <= MIE_MAX_TOP_K,
+  MIE_CHECK_ARG(tokens >= 0 && width >= 1 && width <= MIE_MAX_PRODUCT && ff >= 1 && ff <= 1 << 30 && experts >= 1 &&
+                    experts <= MIE_MAX_EXPERTS && top_k >= 1 && top_k <= MIE_MAX_TOP_K,
                 "invalid sizes: %d tokens of %d, %d of %d experts of %d", tokens, width, top_k, experts, ff);
   MIE_CHECK_ARG((long long)tokens * top_k < (1ll << 30), "too many (token, expert) pairs");
   MIE_CHECK_ARG(ldx >= width && gate_up_row >= width && down_row >= ff && ldy >= width && (!residual || ldr >= width),

@@ -150,7 +150,8 @@ extern "C" int mie_fused_linear(const void* x, int64_t ldx, const void* w, int64
                                 int32_t activation, int32_t gated, int32_t* status, void* stream_) {
   cudaStream_t stream = (cudaStream_t)stream_;
   MIE_CHECK_ARG(x && w && y, "null pointer");
-  MIE_CHECK_ARG(m >= 0 && n >= 1 && k >= 1 && n <= (1 << 30), "invalid product %d x %d x %d", m, n, k);
+  MIE_CHECK_ARG(m >= 0 && n >= 1 && k >= 1 && m <= MIE_MAX_PRODUCT && n <= (1 << 30) && k <= MIE_MAX_PRODUCT,
+                "invalid product %d x %d x %d", m, n, k);
   MIE_CHECK_ARG(ldx >= k && ldw >= k && ldy >= n && (!residual || ldr >= n), "a row is longer than its stride");
   MIE_CHECK_ARG(activation >= MIE_ACT_NONE && activation <= MIE_ACT_RELU, "unknown activation %d", activation);
   if (m == 0) return MIE_OK;

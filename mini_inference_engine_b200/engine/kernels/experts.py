@@ -8,7 +8,7 @@ import functools
 import torch
 
 from ... import _lib
-from .linear import activation_code, check_rows, check_sizes, check_status
+from .linear import MAX_PRODUCT, activation_code, check_rows, check_sizes, check_status
 
 MAX_EXPERTS = 1024  # MIE_MAX_EXPERTS
 MAX_TOP_K = 32      # MIE_MAX_TOP_K
@@ -95,7 +95,7 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate_u
     code, device = activation_code(activation), x.device
     (tokens, width), (experts, double_ff, _), top_k = x.shape, gate_up.shape, int(ids.shape[1])
     ff = double_ff // 2
-    check_sizes(tokens, width, experts, double_ff, top_k)
+    check_sizes(tokens, width, experts, double_ff, top_k, most=MAX_PRODUCT)
     if not (1 <= experts <= MAX_EXPERTS and 1 <= top_k <= MAX_TOP_K and width >= 1 and ff >= 1):
         raise ValueError(f"expert_mlp takes up to {MAX_EXPERTS} experts, {MAX_TOP_K} of them a token, and rows of one entry or "
                          f"more, not {top_k} of {experts} experts of {width} x {ff}")

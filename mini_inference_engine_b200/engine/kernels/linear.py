@@ -96,11 +96,14 @@ def check_rows(name: str, tensor: torch.Tensor, shape: tuple[int, ...], device: 
     return leading[0] if leading else width, leading[1] if len(leading) > 1 else matrix
 
 
-def check_sizes(*sizes: int) -> None:
-    """The library takes sizes of 32 bits."""
+MAX_PRODUCT = (1 << 31) - 4096  # MIE_MAX_PRODUCT
 
-    if max(sizes) >= 1 << 31 or min(sizes) < -1 << 31:
-        raise ValueError(f"sizes up to 2^31 - 1, not {max(sizes, key=abs)}")
+
+def check_sizes(*sizes: int, most: int = (1 << 31) - 1) -> None:
+    """The library takes sizes of 32 bits, of products up to ``MAX_PRODUCT``."""
+
+    if max(sizes) > most or min(sizes) < -1 << 31:
+        raise ValueError(f"sizes up to {most}, not {max(sizes, key=abs)}")
 
 
 def check_status(status: torch.Tensor, device: torch.device) -> None:
@@ -120,7 +123,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     code, device = activation_code(activation), x.device
     rows, k = x.shape
     n = weight.shape[0]
-    check_sizes(rows, n, k)
+    check_sizes(rows, n, k, most=MAX_PRODUCT)
     ldx, _ = check_rows("x", x, (rows, k), device)
     ldw, _ = check_rows("weight", weight, (n, k), device)
     if bias is not None:

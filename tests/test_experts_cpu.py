@@ -121,3 +121,14 @@ def test_refusals_of_pools():
     with pytest.raises(ValueError, match="pairs"):
         expert_mlp(torch.zeros(1, 16).bfloat16().expand(1 << 26, 16), ids, weights, torch.zeros(4, 16, 16).bfloat16(),
                    torch.zeros(4, 16, 8).bfloat16(), status=status)
+
+
+def test_sizes_whose_tiles_pass_32_bits_are_refused(lib):
+    """Tiles are counted in 32 bits, past the last row, column and block of k."""
+
+    most = (1 << 31) - 4096
+    for wrong in ({"width": most + 1, "ldx": 1 << 31, "gate_up_row": 1 << 31, "ldy": 1 << 31},
+                  {"ff": (1 << 30) + 1, "down_row": 1 << 31}):
+        assert experts_call(lib, tokens=1, scratch_bytes=1 << 60, **wrong) == -1, wrong
+        assert lib.mie_expert_scratch_bytes(1, 2, 4, wrong.get("width", 16), wrong.get("ff", 8)) == 0
+    assert experts_call(lib, width=most, ldx=most, gate_up_row=most, ldy=most) == 0

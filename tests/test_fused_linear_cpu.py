@@ -45,3 +45,13 @@ def test_refusals_of_the_c_entry(lib):
     for wrong in ({"x": 0}, {"m": -1}, {"n": 0}, {"k": 0}, {"ldx": 7}, {"ldw": 7}, {"ldy": 7}, {"activation": 4},
                   {"activation": -1}, {"residual": residual, "ldr": 7}):
         assert call(lib, **{"m": 0, **wrong}) == -1, wrong
+
+
+def test_sizes_whose_tiles_pass_32_bits_are_refused(lib):
+    """Tiles are counted in 32 bits, past the last row, column and block of k."""
+
+    most = (1 << 31) - 4096
+    for wrong in ({"m": most + 1}, {"m": (1 << 31) - 1}, {"k": most + 1, "ldx": most + 1, "ldw": most + 1},
+                  {"k": (1 << 31) - 1, "ldx": 1 << 31, "ldw": 1 << 31}, {"n": (1 << 30) + 1, "ldy": 1 << 31}):
+        assert call(lib, **wrong) == -1, wrong
+    assert call(lib, m=0, k=most, ldx=most, ldw=most) == 0
