@@ -8,7 +8,7 @@ import functools
 import torch
 
 from ... import _lib
-from .linear import MAX_PRODUCT, activation_code, check_rows, check_sizes, check_status
+from .linear import MAX_PRODUCT, activation_code, check_rows, check_sizes, check_status, check_tangents
 
 MAX_EXPERTS = 1024  # MIE_MAX_EXPERTS
 MAX_TOP_K = 32      # MIE_MAX_TOP_K
@@ -50,6 +50,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scores: str = "softmax", 
     NaN."""
 
     del status  # every input is valid on the device
+    check_tangents(logits, bias)
     check_sizes(*logits.shape, top_k, groups, top_groups, group_best)
     if logits.ndim != 2 or logits.dtype not in _lib.DTYPE_CODES:
         raise ValueError("route_experts takes CUDA logits [tokens, experts] in bf16, fp16 or fp32")
@@ -92,6 +93,7 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate_u
     if x.ndim != 2 or gate_up.ndim != 3 or down.ndim != 3 or ids.ndim != 2:
         raise ValueError("expert_mlp takes x [tokens, width], ids [tokens, top_k], gate_up [experts, 2 ff, width] and "
                          "down [experts, width, ff]")
+    check_tangents(x, weights, gate_up, down, residual)
     code, device = activation_code(activation), x.device
     (tokens, width), (experts, double_ff, _), top_k = x.shape, gate_up.shape, int(ids.shape[1])
     ff = double_ff // 2

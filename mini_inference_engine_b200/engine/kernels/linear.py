@@ -5,6 +5,7 @@ and of any number of rows with bias, activation or gate, and residual in the epi
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from ... import _lib
 
@@ -106,6 +107,15 @@ def check_sizes(*sizes: int, most: int = (1 << 31) - 1) -> None:
         raise ValueError(f"sizes up to {most}, not {max(sizes, key=abs)}")
 
 
+def check_tangents(*operands: torch.Tensor | None) -> None:
+    """Refuses what forward-mode differentiation follows: its tangent would be lost.  There are none outside its levels."""
+
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in operands):
+        raise ValueError("an operand carries a forward-mode derivative: this operator has none")
+
+
 def check_status(status: torch.Tensor, device: torch.device) -> None:
     if status.dtype is not torch.int32 or status.device != device or status.numel() < 1:
         raise ValueError(f"status must be an int32 word on {device}")
@@ -120,6 +130,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
 
     if x.ndim != 2 or weight.ndim != 2:
         raise ValueError("fused_linear takes rows [rows, k] and a weight [n, k]")
+    check_tangents(x, weight, bias, residual)
     code, device = activation_code(activation), x.device
     rows, k = x.shape
     n = weight.shape[0]

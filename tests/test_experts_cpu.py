@@ -132,3 +132,28 @@ def test_sizes_whose_tiles_pass_32_bits_are_refused(lib):
         assert experts_call(lib, tokens=1, scratch_bytes=1 << 60, **wrong) == -1, wrong
         assert lib.mie_expert_scratch_bytes(1, 2, 4, wrong.get("width", 16), wrong.get("ff", 8)) == 0
     assert experts_call(lib, width=most, ldx=most, gate_up_row=most, ldy=most) == 0
+
+
+def test_tangents_are_refused():
+    """Forward-mode derivatives would be lost."""
+
+    from torch.autograd import forward_ad
+
+    x, ids, weights = torch.zeros(2, 16).bfloat16(), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, 2)
+    gate_up, down, status = torch.zeros(4, 16, 16).bfloat16(), torch.zeros(4, 16, 8).bfloat16(), torch.zeros(1, dtype=torch.int32)
+    given = {"x": x, "weights": weights, "gate_up": gate_up, "down": down, "residual": x.clone()}
+    logits, bias = torch.zeros(2, 8), torch.zeros(8)
+    for grad in (True, False):
+        with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+            for name, value in given.items():
+                dual = forward_ad.make_dual(value, torch.ones_like(value))
+                with pytest.raises(ValueError, match="derivative"):
+                    expert_mlp(ids=ids, status=status, **{**given, name: dual})
+            with pytest.raises(ValueError, match="derivative"):
+                route_experts(forward_ad.make_dual(logits, torch.ones_like(logits)), 2)
+            with pytest.raises(ValueError, match="derivative"):
+                route_experts(logits, 2, bias=forward_ad.make_dual(bias, torch.ones_like(bias)))
+            with pytest.raises(ValueError, match="CUDA"):  # without a tangent nothing is in the way
+                route_experts(logits, 2, bias=bias)
+    with pytest.raises(ValueError, match="derivative"):
+        torch.func.jvp(lambda z: route_experts(z, 2)[1], (logits,), (logits,))

@@ -55,3 +55,16 @@ def test_sizes_whose_tiles_pass_32_bits_are_refused(lib):
                   {"k": (1 << 31) - 1, "ldx": 1 << 31, "ldw": 1 << 31}, {"n": (1 << 30) + 1, "ldy": 1 << 31}):
         assert call(lib, **wrong) == -1, wrong
     assert call(lib, m=0, k=most, ldx=most, ldw=most) == 0
+
+
+@pytest.mark.parametrize("which", ["x", "weight", "bias", "residual"])
+def test_tangents_are_refused(which):
+    """Forward-mode derivatives would be lost."""
+
+    from torch.autograd import forward_ad
+
+    given = {"x": rows(2, 8), "weight": rows(4, 8), "bias": rows(1, 4)[0], "residual": rows(2, 4)}
+    with forward_ad.dual_level():
+        given[which] = forward_ad.make_dual(given[which], torch.ones_like(given[which]))
+        with pytest.raises(ValueError, match="derivative"):
+            fused_linear(**given, status=torch.zeros(1, dtype=torch.int32))
