@@ -297,8 +297,8 @@ def view4_arg(tensor: torch.Tensor | None) -> View4T:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def stream_arg(device: torch.device | None = None) -> c_void_p:
-    if _raw_stream is None or device is None or device.index is None:
+def stream_arg(device: torch.device | str | int | None = None) -> c_void_p:
+    if _raw_stream is None or not isinstance(device, torch.device) or device.index is None:
         return c_void_p(torch.cuda.current_stream(device).cuda_stream)
     return c_void_p(_raw_stream(device.index))
 
