@@ -442,6 +442,66 @@ def test_weights_routed_by_the_call_before(device):
             assert torch.equal(out, expected)
 
 
+@pytest.mark.parametrize("tokens", [1, 5, 16, 17, 32])
+@pytest.mark.parametrize("experts,top_k,width,ff", [(4, 2, 512, 2048), (40, 8, 256, 1024), (8, 2, 4096, 512), (5, 2, 72, 4000)])
+def test_few_rows_sums_of_whole_numbers_are_exact(tokens, experts, top_k, width, ff, device):
+    """Up to 32 tokens no sum is held in less than fp32, within an expert or over them.
+
+    Rows of x have one entry that is not zero, so that gates and ups are whole numbers up to 8 and hidden values (a rounding to
+    bf16 of whole numbers up to 64) are exact; so is every partial sum, at most 2 top_k ff 64 16 <= 2^24.  The
+    residual takes the sum rounded to bf16 away, and what is left is rounded once."""
+
+    torch.manual_seed(tokens + width)
+    whole = lambda most, *shape: torch.randint(-most, most + 1, shape, device=device).to(torch.bfloat16)  # noqa: E731
+    gate_up, down = whole(8, experts, 2 * ff, width), whole(16, experts, width, ff)
+    x = torch.zeros(tokens, width, dtype=torch.bfloat16, device=device)
+    x[torch.arange(tokens, device=device), torch.randint(0, width, (tokens,), device=device)] = 1.0
+    ids = torch.argsort(torch.rand(tokens, experts, device=device), dim=1)[:, :top_k].to(torch.int32)
+    weights = torch.randint(1, 3, (tokens, top_k), device=device).float()
+    exact = torch.zeros(tokens, width, dtype=torch.float64, device=device)
+    for j in range(top_k):
+        for t in range(tokens):
+            e = int(ids[t, j])
+            z = gate_up[e].double() @ x[t].double()
+            exact[t] += weights[t, j].double() * (down[e].double() @ (z[:ff] * z[ff:]))
+    rounded = exact.to(torch.bfloat16)
+    status = torch.zeros(1, dtype=torch.int32, device=device)
+    out = expert_mlp(x, ids, weights, gate_up, down, activation="none", residual=-rounded, status=status)
+    assert torch.equal(out, (exact - rounded.double()).to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("tokens", [33, 200, 700])
+@pytest.mark.parametrize("width", [128, 1000])
+def test_rows_of_pairs_have_an_exponent_per_run(tokens, width, device):
+    """Channels in runs of 32 whose magnitudes lie up to 2^60 apart: a pair's row keeps fp16's precision in each of them.
+
+    With one entry of x and one hidden value that are not zero a pair's row is exact before it becomes fp16 (a value is off by
+    2^-11 of it, or by 2^-25 2^-14 of its run's largest where it is subnormal).  The residual takes the row rounded to bf16 away,
+    so that the last rounding is one of what is left."""
+
+    torch.manual_seed(tokens + width)
+    experts, ff = 6, 64
+    scale = 2.0 ** torch.randint(-30, 31, ((width + 31) // 32,), device=device).double().repeat_interleave(32)[:width]
+    gate_up = torch.zeros(experts, 2 * ff, width, dtype=torch.bfloat16, device=device)
+    gate_up[:, 3, 5] = 1.0
+    gate_up[:, ff + 3, 5] = 1.0
+    down = (torch.randn(experts, width, ff, device=device).double() * scale[:, None]).to(torch.bfloat16)
+    x = torch.zeros(tokens, width, dtype=torch.bfloat16, device=device)
+    x[:, 5] = 1.0
+    ids = torch.randint(0, experts, (tokens, 1), device=device, dtype=torch.int32)
+    # 1 + 2^-7: a hidden value of eight bits, so that a row has up to sixteen and is rounded as fp16.
+    weights = torch.full((tokens, 1), 1.0 + 2.0 ** -7, device=device)
+    row = down[ids[:, 0].long(), :, 3].double() * (1.0 + 2.0 ** -7)
+    rounded = row.to(torch.bfloat16)
+    status = torch.zeros(1, dtype=torch.int32, device=device)
+    out = expert_mlp(x, ids, weights, gate_up, down, activation="none", residual=-rounded, status=status).double()
+    runs = torch.nn.functional.pad(row.abs(), (0, -width % 32)).view(tokens, -1, 32).amax(dim=2)
+    bound = 2.0 ** -11 * row.abs() + 2.0 ** -39 * runs.repeat_interleave(32, dim=1)[:, :width]
+    left = row - rounded.double()
+    bound = bound + 2.0 ** -8 * (left.abs() + bound) + 2.0 ** -23 * row.abs()
+    assert_within(out, left, bound)
+
+
 def test_feed_forward_refuses(device):
     x, gate_up, down = torch.zeros(2, 16, device=device).bfloat16(), *pool(4, 16, 8, device)
     ids, weights = torch.zeros(2, 2, dtype=torch.int32, device=device), torch.zeros(2, 2, device=device)

@@ -174,3 +174,32 @@ def test_weights_written_by_a_queued_call(device):
             w = fused_linear(a, eye, status=status)
             out = fused_linear(x, w, status=status)
         assert_within(out, *exact_fused_linear(x, a, None, "none", False, None))
+
+
+def whole_numbers(r, c, most, device):
+    return torch.randint(-most, most + 1, (r, c), device=device).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("m", [1, 16, 24, 64, 100, 256, 1021])
+@pytest.mark.parametrize("n,k", [(256, 12288), (1000, 9728), (520, 4104), (96, 2055)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_sums_of_whole_numbers_are_exact(m, n, k, gated, device):
+    """No sum, in parts or whole, is held in less than fp32.
+
+    Operands are whole numbers up to 16, so that every partial sum, whatever the order, is one below k 16^2 + 2 16 < 2^24 and
+    exact in fp32; parts of it pass 2^11, where fp16 and bf16 would lose their last bits.  The residual takes the sum rounded
+    to bf16 away: what is left, at most half a step of the sum (2^-9 of 2^22), is a multiple of a power of two with at most 14
+    bits and is rounded once."""
+
+    torch.manual_seed(m + n + k)
+    x, w = whole_numbers(m, k, 16, device), whole_numbers(n, k, 16, device)
+    bias = whole_numbers(1, n, 16, device)[0]
+    exact = x.double() @ w.double().t() + bias.double()
+    rounded = exact.to(torch.bfloat16)
+    weight, b = w, bias
+    if gated:  # ups of one: the bias alone
+        weight, b = torch.cat([w, torch.zeros_like(w)]), torch.cat([bias, torch.ones_like(bias)])
+    status = torch.zeros(1, dtype=torch.int32, device=device)
+    out = fused_linear(x, weight, b, activation="none", gated=gated, residual=-rounded, status=status)
+    assert torch.equal(out, (exact - rounded.double()).to(torch.bfloat16))
+    assert int(status.item()) == 0
