@@ -496,7 +496,7 @@ int mie_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const voi
  * Projection of bf16 rows with its epilogue: y[m, n] = act(x[m, k] w[n, k]^T + bias[n]) + residual[m, n]; gated: w and
  * bias have 2 n rows, gates first, and y = act(x w_g^T + bias_g) * (x w_u^T + bias_u) + residual.  fp32 sums and epilogue,
  * one rounding to bf16.  bias and residual may be NULL; y may be the residual itself, not x.  Strides in elements, any
- * sizes and alignments.
+ * alignments; m and k up to MIE_MAX_PRODUCT, n up to 2^30.  The order of the sums follows the sizes.
  */
 int mie_fused_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
                      int64_t ldr, void* y, int64_t ldy, int32_t m, int32_t n, int32_t k, int32_t activation,
@@ -506,9 +506,10 @@ int mie_fused_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, con
  * Experts of every token, from its router logits z[experts] (bf16, fp16 or fp32 by `dtype`, row stride `ld`):
  * s = softmax(z) or sigmoid(z), c = s + bias[experts] (fp32, may be NULL), -inf where z is -inf.  With groups > 1, the
  * experts are that many equal runs; the top_groups groups whose group_best (1 or 2) largest c add up to most stay.
- * ids[tokens, top_k]: the experts with the largest c, descending, equal ones by their index, as 64 bits decide;
- * weights: s of those, over their sum if `renormalize` (0 if that is 0), times scale.  A token with a NaN among its
- * logits gets NaN weights.
+ * ids[tokens, top_k]: the experts with the largest c, descending, equal ones by their index.  Without a bias, and with
+ * one group or group_best 1, the order is that of the logits; otherwise that of c as 64 bits compute it, in which for
+ * instance sigmoids of 40 and 41 are equal.  weights: s of those, over their sum if `renormalize` (0 if that is 0),
+ * times scale.  A token with a NaN among its logits gets NaN weights.
  */
 #define MIE_SCORES_SOFTMAX 0
 #define MIE_SCORES_SIGMOID 1
@@ -522,9 +523,15 @@ int mie_route_experts(const void* logits, int64_t ld, int32_t dtype, const float
  * Gated feed-forward of routed experts: y[t] = residual[t] + sum_j weights[t, j] D_e (act(G_e x[t]) * (U_e x[t])) with
  * e = ids[t, j]; gate_up[e] = [G_e; U_e] is [2 ff, width], down[e] = D_e is [width, ff], bf16, strides in elements.
  * weights: contiguous fp32 [tokens, top_k].  An id of -1 is no expert; others outside [0, experts) are skipped and
- * reported (MIE_STATUS_BAD_EXPERT).  fp32 sums; the gated rows are rounded once to bf16 (with their weight) before the
- * down product, y once.  y may be the residual itself, not x.  scratch: mie_expert_scratch_bytes of device memory,
- * 256-byte aligned, in use until the call's work is done.
+ * reported (MIE_STATUS_BAD_EXPERT).  fp32 sums; the gated rows are rounded once to bf16 before the down product, y once.
+ * Which form a call takes goes by its sizes and alignment.  Up to 32 tokens a pair's weight is applied in fp32, after
+ * the down product.  Above, and at any number of tokens where rows of x, gate_up or down do not begin and end on 16-byte
+ * borders, the weight is part of the gated row, before its rounding; and above, with rows that do, a pair's row of the
+ * down product is rounded before the sum to fp16 with an exponent per 32 channels: off by 2^-11 of a value, or by 2^-39
+ * of the largest finite one of its 32.
+ * y may be the residual itself, not x.  width up to MIE_MAX_PRODUCT, ff up to 2^30, tokens x top_k below 2^30.  scratch:
+ * mie_expert_scratch_bytes of device memory (0 for sizes that no call takes), 256-byte aligned, in use until the call's
+ * work is done.
  */
 int64_t mie_expert_scratch_bytes(int32_t tokens, int32_t top_k, int32_t experts, int32_t width, int32_t ff);
 int mie_expert_mlp(const void* x, int64_t ldx, mie_index_t ids, const float* weights, const void* gate_up,

@@ -11,8 +11,8 @@
 //                          lose as much again as by the hidden rows' rounding, as fp32 its rows would be twice the bytes
 //   expert_combine_kernel  adds a token's rows and the residual
 //
-// 8192 tokens of 2048 x 768, 8 of 128 experts (us, one after the other without a launch chain): 14, 304 to 328, 196 to 207, 86.  The products
-// are bound as product_wide.cuh says (the down product also by its 268 MB of rows, which HBM takes beside the weights); the
+// 8192 tokens of 2048 x 768, 8 of 128 experts (us, one after the other without a launch chain): 14, 304 to 328, 196 to 207, 86.
+// The products are bound as product_wide.cuh says (the down product also by its 268 MB of rows, which HBM takes beside the weights); the
 // sum moves its 340 MB at 0.6 of the copy rate.  Together 620 us in a burst, 715 to 780 back to back; the products' floor is 380.
 //
 // A pair's order among its expert's rows is whatever the counters gave; every row of a product is computed by itself, so
@@ -324,7 +324,8 @@ struct Scratch {
     hidden = take((pairs > few ? pairs : few) * ff * 2);
     exponents = take(pairs * exponent_ld(width));
     // Few rows: the parts of the down product, at most one CTA's an SM or one of every tile.
-    const long long tiles = (width + 127) / 128, parts = tokens > kFewRoutedRows ? 0 : (tiles > kMostParts ? tiles : kMostParts) * (tokens > 16 ? 32 : 16) * 128 * 4;
+    const long long tiles = (width + 127) / 128, ctas = tiles > kMostParts ? tiles : kMostParts;
+    const long long parts = tokens > kFewRoutedRows ? 0 : ctas * (tokens > 16 ? 32 : 16) * 128 * 4;
     rows = take(pairs * width * 4 > parts ? pairs * width * 4 : parts);
   }
   long long take(long long bytes) {
@@ -465,8 +466,8 @@ extern "C" int mie_expert_mlp(const void* x, int64_t ldx, mie_index_t ids, const
   }
   const int tile_rows = wide ? kWideRows : kAnyTile;
   const long long tiles = s.most_tiles(pairs, experts, tile_rows);
-  const PlanParams plan{IndexView(ids), pairs, top_k, experts, tile_rows, order, (int*)(base + s.position), (RowTile*)(base + s.tiles),
-                        (int*)(base + s.tile_count), status,
+  const PlanParams plan{IndexView(ids), pairs, top_k, experts, tile_rows, order, (int*)(base + s.position),
+                        (RowTile*)(base + s.tiles), (int*)(base + s.tile_count), status,
                         !ids.is64 && ids.stride1 == 1 && ids.stride0 == top_k && (reinterpret_cast<uintptr_t>(ids.ptr) & 15) == 0};
   if (int rc = launch_plan(plan, stream)) return rc;
   if (!wide) {

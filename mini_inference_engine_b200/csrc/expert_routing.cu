@@ -7,11 +7,13 @@
 // 8, 16 or 32 lanes take a token (32 / lanes of them a warp), runs of V experts a lane, so that the lowest lane that has the
 // largest value has the lowest index.  Every lane sorts its run once; a choice is then one maximum over the token's lanes'
 // heads, and the lane that has it moves on.  Little data and many dependent steps: bound by instruction issue for many tokens
-// and by latency for few.  One token of 128 3.3 us, 30011 of 64 8.0, 4096 of 256 by groups and bias 15.6 (its bytes 0.7; a lane
+// and by latency for few.  One token of 128 3.1 us, 30011 of 64 7.8, 4096 of 256 by groups and bias 16.4 (its bytes 0.7; a lane
 // that scanned its run for every choice took 18.1 of the second, 39.5 of the third with whole rows decided again in 64 bits).
+// With a bias, 4096 of 512 take 65 us and of 1024 260: the runs' 16 and 32 entries a lane fill the registers, 32 spill.
 //
-// The choice is that of 64 bits.  Without a bias, and with groups judged by their best expert, the order of the scores is the
-// order of the logits, which are compared as they are.  Otherwise c is computed in 32 bits with an error below 2^-19 (1 + |c|)
+// Without a bias, and with one group or groups judged by their best expert, the order of the scores is the order of the logits,
+// which are compared as they are.  Otherwise the choice is that of c in 64 bits (where large sigmoids may be equal whose logits
+// are not).  c is computed in 32 bits with an error below 2^-19 (1 + |c|)
 // (approximate exponential and reciprocal 2^-22 each, the argument's rounding, a sum of up to 1024 terms, the bias' addition,
 // of a value in [0, 1] or of c).  Where two values that decide something are nearer than twice that and do not come from
 // equal logits and biases, the choice goes on to whatever is as near, and those candidates are ordered by c in 64 bits (all
@@ -237,7 +239,7 @@ __device__ __noinline__ bool has_rival(const RouteParams& p, const T* row, float
   return __any_sync(kAll, found);
 }
 
-// Descending by (key, low).
+// Descending by (key, low): Batcher's odd-even merge sort.
 template <int V>
 __device__ __forceinline__ void sort_run(uint32_t (&key)[V], uint32_t (&low)[V]) {
 #pragma unroll

@@ -210,7 +210,8 @@ __device__ __forceinline__ void finish_rows(const FewParams& q, uint32_t park, i
       for (int j = 0; j < 4; ++j) o[j] = (kGated ? v[4 * b + j] * u[b][j] : v[4 * b + j]) + r[b][j];
       __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(p.y) + (to0 + first + b * kStep) * p.ldy + channel;
       if (vec_y && valid == 4) {
-        *reinterpret_cast<uint2*>(y) = make_uint2(Mma16816<__nv_bfloat16>::pack(o[0], o[1]), Mma16816<__nv_bfloat16>::pack(o[2], o[3]));
+        *reinterpret_cast<uint2*>(y) =
+            make_uint2(Mma16816<__nv_bfloat16>::pack(o[0], o[1]), Mma16816<__nv_bfloat16>::pack(o[2], o[3]));
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -220,8 +221,8 @@ __device__ __forceinline__ void finish_rows(const FewParams& q, uint32_t park, i
   }
 }
 
-// grid = (tiles, split, tiles of rows), cluster = (1, split) unless the parts meet in global memory.  Without a split, kUp has as many CTAs as run at once, which go
-// through the tiles of all experts without a pause.
+// grid = (tiles, split, tiles of rows), cluster = (1, split) unless the parts meet in global memory.  Without a split, kUp has as
+// many CTAs as run at once, which go through the tiles of all experts without a pause.
 template <int BN, Few kKind, bool kGated>
 __global__ void __launch_bounds__(kFewThreads, FewSmem<BN, kKind>::kCtasPerSm)
     product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const FewParams q) {
@@ -269,7 +270,8 @@ __global__ void __launch_bounds__(kFewThreads, FewSmem<BN, kKind>::kCtasPerSm)
   if (kKind != Few::kDown) chain_wait();
   if (kKind == Few::kUp) {
     chain_release();
-    for (int i = (int)(blockIdx.x * kFewThreads + threadIdx.x); i < q.down_tiles; i += (int)gridDim.x * kFewThreads) q.arrived[i] = 0;
+    for (int i = (int)(blockIdx.x * kFewThreads + threadIdx.x); i < q.down_tiles; i += (int)gridDim.x * kFewThreads)
+      q.arrived[i] = 0;
   }
   const int used = kKind == Few::kDense ? 1 : find_routing(routing, q, kKind == Few::kUp);
 

@@ -178,7 +178,9 @@ __device__ __forceinline__ WideTile wide_tile(const WideParams& q, int index) {
 }
 
 // Where a finishing warp parks four of the 32 sums that a lane has of a chunk.
-__device__ __forceinline__ int parked(int warp, int chunk, int four, int lane) { return ((warp * 4 + chunk) * 8 + four) * 512 + lane * 16; }
+__device__ __forceinline__ int parked(int warp, int chunk, int four, int lane) {
+  return ((warp * 4 + chunk) * 8 + four) * 512 + lane * 16;
+}
 static_assert(kWideFinishers * 4 * 8 * 512 <= wide_stages<true>() * kWideStageBytes, "the ring parks a tile's sums");
 
 template <Rows kRows, bool kGated, bool kDirect>
@@ -485,7 +487,8 @@ __global__ void __launch_bounds__(wide_threads<kRows>(), 1)
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             *reinterpret_cast<float4*>(ring + parked(warp, chunk >> 1, i, lane)) =
-                make_float4(v[i >> 2][4 * (i & 3)], v[i >> 2][4 * (i & 3) + 1], v[i >> 2][4 * (i & 3) + 2], v[i >> 2][4 * (i & 3) + 3]);
+                make_float4(v[i >> 2][4 * (i & 3)], v[i >> 2][4 * (i & 3) + 1], v[i >> 2][4 * (i & 3) + 2],
+                            v[i >> 2][4 * (i & 3) + 3]);
         } else {
           finish(chunk, v);
           if (has_residual && chunk + 2 < n_chunks) load_residual(chunk + 2);
@@ -713,7 +716,8 @@ __global__ void __launch_bounds__(wide_threads<kRows>(), 1)
 #pragma unroll
             for (int w = 0; w < kWords; ++w) {
               const int row = quad * kEach + i, c = 2 * (lane + 32 * w);
-              word[i][w] = *reinterpret_cast<const uint32_t*>(stage + row * kRowBytes + (((c >> 3) ^ (row & 7)) * 16) + (c & 7) * 2);
+              word[i][w] =
+                  *reinterpret_cast<const uint32_t*>(stage + row * kRowBytes + (((c >> 3) ^ (row & 7)) * 16) + (c & 7) * 2);
             }
           }
 #pragma unroll
@@ -844,7 +848,8 @@ int launch_wide(const WeightMaps& maps, const CUtensorMap& map_x, const WidePara
   if (int rc = configure_wide<kRows, kGated, kDirect>()) return rc;
   const long long most = parts > 1 ? most_tiles : sm_count() / 2;
   cudaLaunchAttribute attr[2];
-  const cudaLaunchConfig_t config = wide_config<kRows, kGated, kDirect>(attr, (int)(most_tiles < most ? most_tiles : most), parts, stream);
+  const cudaLaunchConfig_t config =
+      wide_config<kRows, kGated, kDirect>(attr, (int)(most_tiles < most ? most_tiles : most), parts, stream);
   prefer_shared_carveout(reinterpret_cast<const void*>(product_wide_kernel<kRows, kGated, kDirect>));
   MIE_CUDA(cudaLaunchKernelEx(&config, product_wide_kernel<kRows, kGated, kDirect>, maps, map_x, q));
   MIE_LAUNCH_CHECK("product_wide_kernel");

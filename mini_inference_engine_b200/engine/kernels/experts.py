@@ -45,8 +45,9 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scores: str = "softmax", 
     ``s = softmax(logits)`` or ``sigmoid(logits)``; the choice goes by ``s + bias`` (fp32 ``[experts]``, for balance), the
     weights are ``s`` of the chosen, over their sum with ``renormalize``, times ``scale``.  With ``groups`` the experts are
     that many equal runs, of which the ``top_groups`` whose ``group_best`` (1 or 2) best choices add up to most are chosen
-    from.  Best first, equal choices by their index; values that 32 bits do not tell apart are decided in 64.  A
-    logit of ``-inf`` masks an expert: it comes after all others, with weight 0.  A NaN logit makes the token's weights
+    from.  Best first, equal choices by their index.  Without ``bias``, and without groups or with ``group_best`` 1, the order
+    is that of the logits; otherwise that of the choices in 64 bits (in which sigmoids of 40 and 41, for instance, are equal).
+    A logit of ``-inf`` masks an expert: it comes after all others, with weight 0.  A NaN logit makes the token's weights
     NaN."""
 
     del status  # every input is valid on the device
@@ -74,9 +75,9 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scores: str = "softmax", 
         return ids, weights
     with _lib.on_device(device):
         _lib.check(_lib.load().mie_route_experts(
-            logits.data_ptr(), logits.stride(0) if tokens > 1 else experts, _lib.DTYPE_CODES[logits.dtype], None if bias is None else bias.data_ptr(),
-            SCORES[scores], tokens, experts, top_k, groups, top_groups, group_best, int(renormalize), float(scale),
-            ids.data_ptr(), weights.data_ptr(), _lib.stream_arg(device)))
+            logits.data_ptr(), logits.stride(0) if tokens > 1 else experts, _lib.DTYPE_CODES[logits.dtype],
+            None if bias is None else bias.data_ptr(), SCORES[scores], tokens, experts, top_k, groups, top_groups,
+            group_best, int(renormalize), float(scale), ids.data_ptr(), weights.data_ptr(), _lib.stream_arg(device)))
     return ids, weights
 
 
